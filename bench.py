@@ -447,7 +447,7 @@ def main():
     ap.add_argument("--only", choices=["tracker", "mapper", "trained"], default=None, help="diagnostics: run only one half (the JSON line is then NOT the contract metric)")
     ap.add_argument("--cu-split", type=int, default=0, help="EXPERIMENT (round 6): the tracker's stream on this many dedicated compute units "
                     "(hipExtStreamCreateWithCUMask, mask bits 0..N-1: spread evenly over the 8 XCDs) and the mapper's stream on the remaining ones, instead of a "
-                    "high-priority tracker stream sharing all 256; 0 = off")
+                    "tracker stream sharing all 256; 0 = off")
     ap.add_argument("--mp-bands", choices=["off", "equal", "balanced"], default="off",
                     help="N > 1, --mp-mode tiles: `off` = super-tiles dealt round-robin + all-gather of the image (rounds 3-4, the rehearsed default); `equal` / "
                          "`balanced` (round 5) = contiguous bands of 32-pixel rows per rank + a halo exchange of 2 x 10 rows (0.4 MB instead of 13.7 MB per rank); "

@@ -2618,22 +2618,17 @@ int gsicp_stream_destroy(void* stream) {
 
 gsicp_gicp* gsicp_gicp_create(void) {
     gsicp_gicp* g = new gsicp_gicp();
-    // The tracker is the latency-critical half (one frame = a short dependent chain of small kernels); the mapper it shares the GPU
-    // with is throughput work.  Highest stream priority lets the tracker's waves go ahead of queued mapper workgroups.
-    int prio_lo = 0, prio_hi = 0;
-    (void)hipDeviceGetStreamPriorityRange(&prio_lo, &prio_hi);
-    const char* pe = std::getenv("GSICP_TRACKER_PRIORITY");   // "0" = default priority (A/B switch for measurements)
-    if (pe && pe[0] == '0') prio_hi = prio_lo = 0;
+    // The stream has the DEFAULT priority: with the mapper's stream at another one, work of the two has been seen to hang on this platform, and a higher
+    // priority for the tracker measured no effect on either half.
     // GSICP_TRACKER_CU_MASK="first:count" (round 6 experiment, default off): the tracker's stream on `count` dedicated compute units starting at mask bit
     // `first` (hipExtStreamCreateWithCUMask; on a multi-XCD part consecutive mask bits go round the XCDs, so a prefix is spread evenly over the eight) —
     // its 33 workgroups then never queue behind mapper waves on those CUs when the mapper's stream carries the complement (gsicp_stream_create_cu_mask).
-    // A masked stream has no priority argument: the two are alternatives.
     const char* cm = std::getenv("GSICP_TRACKER_CU_MASK");
     int cu_first = 0, cu_count = 0;
     if (cm && std::sscanf(cm, "%d:%d", &cu_first, &cu_count) == 2 && cu_count > 0) {
         g->stream = (hipStream_t)gsicp_stream_create_cu_mask(cu_first, cu_count);
         if (!g->stream) { delete g; return nullptr; }
-    } else if (hipStreamCreateWithPriority(&g->stream, hipStreamNonBlocking, prio_hi) != hipSuccess) {
+    } else if (hipStreamCreateWithFlags(&g->stream, hipStreamNonBlocking) != hipSuccess) {
         g_last_error = "hipStreamCreate failed (no HIP device?)";
         delete g;
         return nullptr;

@@ -126,7 +126,7 @@ def _compile_tree(tree, src, dst, dfile):
 
 def main_fused():
     out = os.path.join(HERE, "_ref", "refpy_fused")
-    if not os.path.isdir(REF):
+    if not os.path.exists(os.path.join(REF, "mp_Mapper.py")):
         print(f"make_refpy --fused: {REF} not present (GPU box) — keeping whatever is under {out}")
         return 0
     srcs = [f for f in FILES if os.path.exists(os.path.join(REF, f))]
@@ -157,7 +157,7 @@ def main_fused():
 
 
 def main():
-    if not os.path.isdir(REF):
+    if not os.path.exists(os.path.join(REF, "mp_Mapper.py")):
         print(f"make_refpy: {REF} not present (GPU box) — keeping whatever is under {OUT}")
         return 0
     srcs = [f for f in FILES if os.path.exists(os.path.join(REF, f))]

@@ -75,6 +75,11 @@ SIGNATURES = {
                                        c_void_p, c_int, c_void_p, ctypes.c_uint, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gsicp_adam_step_sparse": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float, c_float,
                                        c_void_p, c_int, c_void_p, ctypes.c_uint, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gsicp_adamw_step": (c_int, [c_int] + [c_void_p] * 9 + [c_double, c_double, c_double, c_int, c_void_p, c_void_p, c_void_p]),
+    "gsicp_adamw_step_8bit": (c_int, [c_int] + [c_void_p] * 9 + [c_double, c_double, c_double, c_int, ctypes.c_uint, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gsicp_adamw_decode": (c_int, [c_int] + [c_void_p] * 5 + [c_int, c_void_p]),
+    "gsicp_grad_norm_scratch_bytes": (c_size_t, [c_int]),
+    "gsicp_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_void_p]),
     "gsicp_stream_create_cu_mask": (c_void_p, [c_int, c_int]),
     "gsicp_stream_destroy": (c_int, [c_void_p]),
     "gsicp_gicp_create": (c_void_p, []),
@@ -122,6 +127,15 @@ SIGNATURES = {
     "gsicp_debug_wave_sort": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gsicp_gicp_barrier_retries": (c_int, [c_void_p]),
 }
+
+
+
+class AdamWDevice(ctypes.Structure):
+    """gsicp_adamw_device: what a captured step reads from device memory."""
+    _fields_ = [("lr_dev", c_void_p), ("step_dev", c_void_p), ("bump_step", c_int), ("guard_count", c_void_p), ("guard_limit", ctypes.c_uint),
+                ("skipped", c_void_p), ("live_rows", c_void_p), ("row_width", c_void_p), ("row_freeze", c_void_p), ("group_frozen", c_void_p),
+                ("grad_rows", c_void_p)]
+
 
 _lib = None
 

@@ -19,6 +19,7 @@ SOURCES = [
     ("mapper_ops.hip", []),
     ("frontend.hip", ["-ffp-contract=off"]),
     ("gicp.hip", ["-ffp-contract=off"]),
+    ("adamw.hip", ["-ffp-contract=off"]),   # the codes of 8-bit moments are reproducible against the written formulas
 ]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 — some forms of them have given wrong results on this platform now and then, without an error.  (The host
 # pass of hipcc warns that it does not know the feature: harmless.)

@@ -131,7 +131,10 @@ class GaussianStore:
         groups = [{"params": [self.params[k]], "lr": float(lrs[k]), "name": k} for k in PARAM_NAMES]
         self.optimizer = optimizer_cls(groups, **kw)
         # the moments live in the store from the first step on (a lazily created zeros_like() would sit outside it)
-        fused = hasattr(self.optimizer, "capturable") and type(self.optimizer).__name__ == "FusedAdam"
+        if getattr(self.optimizer, "state_bits", 32) != 32:
+            self.optimizer = None
+            raise RuntimeError("GaussianStore.attach: the store's moments are 32-bit (rows of 8-bit ones cannot move between blocks that share an exponent)")
+        fused = hasattr(self.optimizer, "capturable") and type(self.optimizer).__name__ in ("FusedAdam", "FusedAdamW")
         shared_step = torch.zeros((), dtype=torch.int32, device=self.device) if (fused and self.optimizer.capturable) else None
         for k in PARAM_NAMES:
             if fused:

@@ -72,7 +72,7 @@ def torch_activations(p, live_rows=None):
 
 class MapperIterationGraph:
     """params: dict of raw leaf tensors (means3D, shs, opacities, scales, rotations) with requires_grad;
-    optimizer: FusedAdam(capturable=True) over them;  capacity: upper bound for the number of (Gaussian, tile) duplicates
+    optimizer: FusedAdam(capturable=True) or FusedAdamW(capturable=True) over them;  capacity: upper bound for the number of (Gaussian, tile) duplicates
     (e.g. 1.5x the count of an eager forward; `overflowed()` tells when it was too small, `ensure_capacity()` enlarges it and re-captures)."""
 
     def __init__(self, params, optimizer, image_height, image_width, tanfovx, tanfovy, sh_degree, capacity, bg=None, lambda_dssim=0.2,
@@ -125,7 +125,8 @@ class MapperIterationGraph:
         # radii as its row mask.  Needs the in-kernel activations (raw parameters: no separate activation backward reading those rows) and a rasteriser
         # whose own gradient handling touches visible rows only (plain; tile-sharded with the static exchange — NOT the dense keyframe-parallel
         # all-reduce).  GSICP_SPARSE_GRADS=0 switches it off (A/B).  A grad_hook sees undefined values in culled rows: mask by `radii > 0`.
-        self._sparse = bool(fused and os.environ.get("GSICP_SPARSE_GRADS", "1") != "0")
+        # An optimiser that clips by the global norm reads every row: dense then.
+        self._sparse = bool(fused and os.environ.get("GSICP_SPARSE_GRADS", "1") != "0" and getattr(optimizer, "max_grad_norm", None) is None)
         if self._sparse:
             rs = rs._replace(sparse_grads=True)
         self.rasterizer = rasterizer_factory(rs) if rasterizer_factory is not None else GaussianRasterizer(rs)

@@ -9,8 +9,19 @@ not supported (the reference does not use them).
 memory, so that ``step()`` can be captured in a HIP graph and replayed (gs_icp_slam_amd/graph.py).  ``state[p]["step"]``
 is then an int32 device tensor shared by the parameters that were first stepped together; after changing a group's
 ``lr`` call ``sync_lr()`` (outside capture) to push the new values to the device.
+
+Beside it, for parameters of any number and of f32, bf16 or f16 (no reference counterpart: the reference trains with torch.optim.Adam):
+
+    norm = grad_norm(grads)                                               # 2-norm over all of them, a device scalar
+    adamw_step(params, grads, exp_avgs, exp_avg_sqs, lr=..., step=t)      # torch.optim.AdamW's step, one launch per 40 tensors
+    adamw_step_8bit(params, grads, moments, block_exps, lr=..., step=t)   # the same with both moments in 8 bits
+    exp_avgs, exp_avg_sqs = decode_moments(moments, block_exps)           # what 8-bit moments stand for
+
+and `FusedAdamW`, the optimiser over them.  `max_norm=` clips by the global norm inside the step: the factor never leaves the device and the gradients are not rewritten.
 """
+import array
 import ctypes
+import operator
 
 import torch
 
@@ -241,3 +252,348 @@ class FusedAdam(torch.optim.Optimizer):
                     LR = (ctypes.c_float * n)(*[t[4] for t in chunk])
                     _lib.check(lib.gsicp_adam_step(n, P, G, M, V, N, LR, b1, b2, eps, step, stream), "gsicp_adam_step")
         return loss
+
+
+# ------------------------------------------------------------------------------------------------ AdamW over many tensors
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_BLOCK = 128                       # elements per base exponent of 8-bit moments
+_numel, _dtype, _device = torch.Tensor.numel, operator.attrgetter("dtype"), operator.attrgetter("device")
+
+
+def _addresses(tensors):
+    return array.array("Q", map(torch.Tensor.data_ptr, tensors))
+
+
+def _at(a):
+    """Address of an array.array's items (the array must outlive the call), or None."""
+    return None if a is None else a.buffer_info()[0]
+
+
+def _check_tensors(what, name, tensors, device, dtypes=None, numels=None):
+    """Lists of contiguous tensors on one HIP device; -> their dtypes.  Works on whole lists: a step over hundreds of small tensors is bound by the host."""
+    for d in set(map(_device, tensors)):
+        if d != device or not device.type == "cuda":
+            raise RuntimeError(f"{what} (gfx950): {name} must live on one HIP device (found {d}); there is no CPU path")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise RuntimeError(f"{what}: {name} must be contiguous")
+    found = list(map(_dtype, tensors))
+    if dtypes is not None and found != dtypes:
+        raise RuntimeError(f"{what}: {name} have the wrong dtype ({', '.join(sorted({str(t) for t in set(found) - set(dtypes)} or {'mixed up'}))})")
+    if numels is not None and list(map(_numel, tensors)) != numels:
+        raise RuntimeError(f"{what}: {name} have the wrong number of elements")
+    return found
+
+
+def _codes(what, name, dtypes):
+    try:
+        return array.array("i", map(_DTYPE_CODE.__getitem__, dtypes))
+    except KeyError as e:
+        raise RuntimeError(f"{what}: {name} must be float32, bfloat16 or float16 (found {e.args[0]})") from None
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _doubles(what, name, value, n):
+    if isinstance(value, (int, float)):
+        return array.array("d", [value]) * n
+    a = array.array("d", value)
+    if len(a) != n:
+        raise RuntimeError(f"{what}: {name} is a number or one per tensor ({len(a)} for {n} tensors)")
+    return a
+
+
+def _norm_launch(what, addresses, numels, codes, device, max_norm):
+    """-> f32[2] on the device: the norm and the clip factor (1 without a max_norm)."""
+    if max_norm is None:
+        max_norm = 0.0
+    elif not max_norm > 0.0:
+        raise RuntimeError(f"{what}: max_norm must be positive")
+    lib = _lib.load()
+    n = len(addresses)
+    out = torch.empty(2, dtype=torch.float32, device=device)
+    scratch = torch.empty(int(lib.gsicp_grad_norm_scratch_bytes(n)), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        _lib.check(lib.gsicp_grad_norm(n, _at(addresses), _at(numels), _at(codes), float(max_norm), out.data_ptr(), scratch.data_ptr(), _stream(device)), "gsicp_grad_norm")
+    return out
+
+
+def grad_norm(tensors):
+    """2-norm over all elements of `tensors` (f32, bf16 or f16, mixed, any sizes, contiguous, one device) as a 0-dim f32 tensor on their device; nothing synchronises.
+    Squares and sums are taken in double and in a fixed order: the same tensors give the same bits."""
+    tensors = list(tensors)
+    if not tensors:
+        raise RuntimeError("grad_norm: no tensors")
+    device = tensors[0].device
+    codes = _codes("grad_norm", "tensors", _check_tensors("grad_norm", "tensors", tensors, device))
+    return _norm_launch("grad_norm", _addresses(tensors), array.array("q", map(_numel, tensors)), codes, device, None)[0]
+
+
+def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, betas, eps, step, max_norm=None, norm=None, seed=0, place=None, device_form=None):
+    """Checks, lays out and launches a step of either form; -> the norm and clip factor (f32[2] on the device) or None.  norm: one taken before (max_norm is then not
+    looked at); device_form(n): the gsicp_adamw_device of a captured step, and what it points to."""
+    n = len(params)
+    device = params[0].device
+    if not len(grads) == len(first) == len(second) == n or (masters is not None and len(masters) != n):
+        raise RuntimeError(f"{what}: {n} parameters, {len(grads)} gradients, {len(first)} and {len(second)} moments" + ("" if masters is None else f", {len(masters)} masters"))
+    dtypes = _check_tensors(what, "parameters", params, device)
+    numels = list(map(_numel, params))
+    _check_tensors(what, "gradients", grads, device, dtypes, numels)
+    codes = _codes(what, "parameters", dtypes)
+    if bits == 32:
+        f32 = [torch.float32] * n
+        _check_tensors(what, "exp_avgs", first, device, f32, numels)
+        _check_tensors(what, "exp_avg_sqs", second, device, f32, numels)
+    else:
+        i16 = [torch.int16] * n
+        _check_tensors(what, "moments", first, device, i16, numels)
+        _check_tensors(what, "block_exps", second, device, i16, [(k + _BLOCK - 1) // _BLOCK for k in numels])
+    master_at = None
+    if masters is not None:
+        given = [m for m in masters if m is not None]
+        _check_tensors(what, "masters", given, device, [torch.float32] * len(given), [k for k, m in zip(numels, masters) if m is not None])
+        master_at = array.array("Q", [0 if m is None else m.data_ptr() for m in masters])
+    param_at, grad_at, first_at, second_at, numel_at = _addresses(params), _addresses(grads), _addresses(first), _addresses(second), array.array("q", numels)
+    lr = None if device_form else _doubles(what, "lr", lr, n)
+    weight_decay = _doubles(what, "weight_decay", weight_decay, n)
+    if norm is None and max_norm is not None:
+        norm = _norm_launch(what, grad_at, numel_at, codes, device, max_norm)
+    clip = None if norm is None else norm.data_ptr() + 4
+    dev, keep = (None, None) if device_form is None else device_form(n)
+    args = [n, _at(param_at), _at(grad_at), _at(master_at), _at(first_at), _at(second_at), _at(numel_at), _at(codes), _at(lr), _at(weight_decay), betas[0], betas[1], eps,
+            int(step)]
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        if bits == 32:
+            _lib.check(lib.gsicp_adamw_step(*args, clip, dev, _stream(device)), "gsicp_adamw_step")
+        else:
+            _lib.check(lib.gsicp_adamw_step_8bit(*args, int(seed) & 0xFFFFFFFF, _at(place), clip, dev, _stream(device)), "gsicp_adamw_step_8bit")
+    del keep
+    return norm
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, max_norm=None):
+    """One torch.optim.AdamW step (amsgrad and maximize off) over all `params`, in place; one launch per 40 tensors.
+
+    params, grads: lists of contiguous f32 / bf16 / f16 tensors on one device, a gradient of its parameter's dtype; exp_avgs, exp_avg_sqs: f32; masters: list of f32 tensors (or
+    None entries) that take the update of 16-bit parameters, which then receive it rounded.  lr, weight_decay: a number, or one per tensor.  step: the 1-based count of this
+    step.  max_norm: clip by the global norm of `grads` (torch.nn.utils.clip_grad_norm_'s factor; the gradients themselves stay as they are) — the norm is returned as a 0-dim
+    tensor, else None.  No tensor that the step writes may overlap another."""
+    params = list(params)
+    if not params:
+        return None
+    norm = _adamw("adamw_step", 32, params, list(grads), masters, list(exp_avgs), list(exp_avg_sqs), lr, weight_decay, betas, eps, step, max_norm)
+    return None if norm is None else norm[0]
+
+
+def adamw_step_8bit(params, grads, moments, block_exps, *, lr, step, seed=0, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, max_norm=None):
+    """adamw_step with both moments in 8 bits: moments[k] int16 of the parameter's number of elements, block_exps[k] int16[ceil(numel / 128)]; all zero before the first step
+    (new_moments_8bit).  Moments are rounded stochastically; the random bits are a function of (seed, step, place in the list, element), so the same call gives the same bits."""
+    params = list(params)
+    if not params:
+        return None
+    norm = _adamw("adamw_step_8bit", 8, params, list(grads), masters, list(moments), list(block_exps), lr, weight_decay, betas, eps, step, max_norm, seed=seed)
+    return None if norm is None else norm[0]
+
+
+def new_moments_8bit(param):
+    """(moments, block_exps) of a parameter before its first step."""
+    return (torch.zeros(param.shape, dtype=torch.int16, device=param.device),
+            torch.zeros((param.numel() + _BLOCK - 1) // _BLOCK, dtype=torch.int16, device=param.device))
+
+
+def decode_moments(moments, block_exps, dtype=torch.float32):
+    """-> (exp_avgs, exp_avg_sqs): the values of 8-bit moments, lists of tensors of the moments' shapes in f32 or bf16 (which holds every code's value exactly)."""
+    moments, block_exps = list(moments), list(block_exps)
+    if not moments:
+        return [], []
+    what = "decode_moments"
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError(f"{what}: dtype is float32 or bfloat16")
+    device, n = moments[0].device, len(moments)
+    _check_tensors(what, "moments", moments, device, [torch.int16] * n)
+    numels = list(map(_numel, moments))
+    _check_tensors(what, "block_exps", block_exps, device, [torch.int16] * n, [(k + _BLOCK - 1) // _BLOCK for k in numels])
+    exp_avgs = [torch.empty(t.shape, dtype=dtype, device=device) for t in moments]
+    exp_avg_sqs = [torch.empty(t.shape, dtype=dtype, device=device) for t in moments]
+    c, b, m, v, k = _addresses(moments), _addresses(block_exps), _addresses(exp_avgs), _addresses(exp_avg_sqs), array.array("q", numels)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().gsicp_adamw_decode(n, _at(c), _at(b), _at(m), _at(v), _at(k), _DTYPE_CODE[dtype], _stream(device)), "gsicp_adamw_decode")
+    return exp_avgs, exp_avg_sqs
+
+
+class FusedAdamW(FusedAdam):
+    """torch.optim.AdamW (amsgrad and maximize off) over any number of f32, bf16 and f16 parameters, one launch per 40 of them with the same betas, eps and step count.
+
+    state_bits      32: state[p] = {"step", "exp_avg", "exp_avg_sq"} (f32; torch's layout, so GaussianStore and the reference's append / prune keep working)
+                    8: state[p] = {"step", "moments", "block_exps"} — adamw_step_8bit's; `moments(p)` gives their values.  A map that grows or is pruned needs 32: its rows
+                    would move between blocks that share an exponent (GaussianStore.attach refuses)
+    master_weights  16-bit parameters keep an f32 copy in state[p]["master"] that takes the update
+    max_grad_norm   clip by the global norm of all gradients of the step; `last_grad_norm` is then a 0-dim device tensor
+    seed            of the stochastic rounding of 8-bit moments
+    capturable      as in FusedAdam: step count and learning rates on the device, the step can be captured and replayed; weight decay, betas and max_grad_norm are part of the
+                    capture.  MapperIterationGraph takes it wherever it takes FusedAdam."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, capturable=False, state_bits=32, master_weights=False, max_grad_norm=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("FusedAdamW: state_bits is 32 or 8")
+        if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("FusedAdamW: lr, eps and weight_decay are not negative, betas in [0, 1)")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError("FusedAdamW: max_grad_norm must be positive")
+        super().__init__(params, lr=lr, betas=betas, eps=eps, capturable=capturable)
+        self.defaults["weight_decay"] = weight_decay
+        for group in self.param_groups:
+            group.setdefault("weight_decay", weight_decay)
+        self.state_bits, self.master_weights, self.max_grad_norm, self.seed = state_bits, bool(master_weights), max_grad_norm, int(seed)
+        self.last_grad_norm = None
+
+    def set_live_rows(self, n_dev):
+        if n_dev is not None and self.state_bits == 8:
+            raise RuntimeError("FusedAdamW(state_bits=8): a capacity-backed map needs 32-bit moments (rows behind the live count would share block exponents with rows that move)")
+        super().set_live_rows(n_dev)
+
+    def set_row_freeze(self, mask, group_names):
+        if mask is not None and self.state_bits == 8:
+            raise RuntimeError("FusedAdamW(state_bits=8): frozen rows need 32-bit moments (they would share block exponents with rows that move)")
+        super().set_row_freeze(mask, group_names)
+
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of a parameter that has been stepped, in f32, whatever state_bits is (a copy with 8, the state itself with 32)."""
+        st = self.state[p]
+        if self.state_bits == 32:
+            return st["exp_avg"], st["exp_avg_sq"]
+        (m,), (v,) = decode_moments([st["moments"]], [st["block_exps"]])
+        return m, v
+
+    def load_state_dict(self, state_dict):
+        """torch's load casts every state tensor to its parameter's dtype; moments, masters and 8-bit codes keep their own here, and parameters that shared a step counter
+        share it again."""
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
+        for i in saved:
+            if any(k not in state_dict["state"].get(i, dict.fromkeys(names)) for k in names):
+                raise ValueError(f"FusedAdamW(state_bits={self.state_bits}): the state was saved with another width of the moments")
+        super().load_state_dict(state_dict)
+        steps = {}
+        for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
+            for k, v in state_dict["state"].get(i, {}).items():
+                if k == "step":
+                    key = (v.data_ptr() if torch.is_tensor(v) else int(v), p.device)
+                    if self.capturable:
+                        v = steps.setdefault(key, torch.full((), int(v), dtype=torch.int32, device=p.device))
+                    else:
+                        v = int(v)
+                elif torch.is_tensor(v):
+                    v = v.detach().to(device=p.device, copy=True)
+                self.state[p][k] = v
+
+    def _new_state(self, p, step):
+        st = self.state[p]
+        st["step"] = step
+        if self.state_bits == 32:
+            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        else:
+            st["moments"], st["block_exps"] = new_moments_8bit(p)
+        if self.master_weights and p.dtype != torch.float32:
+            st["master"] = p.detach().float()
+
+    @torch.no_grad()
+    def step(self, closure=None, step_already_bumped=False):
+        """step_already_bumped: as in FusedAdam.step."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if step_already_bumped and not self.capturable:
+            raise RuntimeError("FusedAdamW.step(step_already_bumped=True) needs capturable=True (a device step counter)")
+        buckets, fresh, place = {}, {}, -1
+        for gi, group in enumerate(self.param_groups):
+            b1, b2 = group["betas"]
+            for pi, p in enumerate(group["params"]):
+                place += 1                                  # counts every parameter: the random bits of one do not depend on which others have a gradient
+                if p.grad is None:
+                    continue
+                if not p.is_cuda:
+                    raise RuntimeError("FusedAdamW (gfx950): parameters must live on the HIP device; there is no CPU path")
+                if p.grad.is_sparse:
+                    raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+                st = self.state[p]
+                if not st:
+                    if self.capturable and p.device not in fresh:
+                        fresh[p.device] = torch.zeros((), dtype=torch.int32, device=p.device)
+                    self._new_state(p, fresh[p.device] if self.capturable else 0)
+                elif self.capturable and not torch.is_tensor(st["step"]):
+                    st["step"] = fresh.setdefault((int(st["step"]), p.device), torch.full((), int(st["step"]), dtype=torch.int32, device=p.device))
+                key = (float(b1), float(b2), float(group["eps"]), st["step"].data_ptr() if self.capturable else int(st["step"]), p.device)
+                buckets.setdefault(key, []).append((p, p.grad.contiguous(), st, gi, pi, place))
+        norm = None
+        if self.max_grad_norm is not None and buckets:
+            if self._grad_rows is not None:
+                raise RuntimeError("FusedAdamW: max_grad_norm reads every gradient row, set_grad_row_mask says some were not written")
+            if len({key[4] for key in buckets}) > 1:
+                raise RuntimeError("FusedAdamW(max_grad_norm): the parameters live on several devices")
+            grads = [t[1] for items in buckets.values() for t in items]
+            device = grads[0].device
+            codes = _codes("FusedAdamW", "gradients", _check_tensors("FusedAdamW", "gradients", grads, device))
+            norm = _norm_launch("FusedAdamW", _addresses(grads), array.array("q", map(_numel, grads)), codes, device, self.max_grad_norm)
+            self.last_grad_norm = norm[0]
+        last_of = {key[3:]: key for key in buckets}         # a device counter is advanced by the last launch that reads it
+        first, second = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
+        for key, items in buckets.items():
+            groups = [self.param_groups[t[3]] for t in items]
+            masters = [t[2].get("master") for t in items]
+            device_form = None
+            if self.capturable:
+                bump = 2 if step_already_bumped else int(last_of[key[3:]] == key)
+                device_form = lambda n, items=items, key=key, bump=bump: self._device_form(items, key, bump)   # noqa: E731
+            _adamw("FusedAdamW", self.state_bits, [t[0] for t in items], [t[1] for t in items], masters if any(m is not None for m in masters) else None,
+                   [t[2][first] for t in items], [t[2][second] for t in items], [float(g["lr"]) for g in groups], [float(g["weight_decay"]) for g in groups], key[:2], key[2],
+                   1 if self.capturable else key[3] + 1, norm=norm, seed=self.seed, place=array.array("i", [t[5] for t in items]), device_form=device_form)
+            if not self.capturable:
+                for t in items:
+                    t[2]["step"] = key[3] + 1
+        return loss
+
+    def _device_form(self, items, key, bump):
+        """The gsicp_adamw_device of one captured launch sequence, and the host arrays it points to."""
+        device, n = key[4], len(items)
+        ids = tuple((t[3], t[4]) for t in items)
+        lrs = [float(self.param_groups[gi]["lr"]) for gi, _ in ids]
+        entry = self._lr_dev.get((ids,) + key[:3])
+        capturing = torch.cuda.is_current_stream_capturing()
+        if entry is None:
+            if capturing:
+                raise RuntimeError("FusedAdamW(capturable): run one step() outside graph capture first (allocates the device lr array)")
+            entry = self._lr_dev[(ids,) + key[:3]] = [torch.tensor(lrs, dtype=torch.float64).to(device), lrs]
+        elif not capturing and entry[1] != lrs:
+            entry[0].copy_(torch.tensor(lrs, dtype=torch.float64))
+            entry[1] = lrs
+        d = _lib.AdamWDevice(lr_dev=entry[0].data_ptr(), step_dev=key[3], bump_step=bump)
+        keep = [d]
+        if self._guard is not None and self._guard[0].device == device:
+            d.guard_count, d.guard_limit, d.skipped = self._guard[0].data_ptr(), self._guard[1], self.skipped_steps.data_ptr()
+        live = self._live_rows if self._live_rows is not None and self._live_rows.device == device else None
+        freeze = self._row_freeze if self._row_freeze is not None and self._row_freeze[0].device == device else None
+        rows = self._grad_rows if self._grad_rows is not None and self._grad_rows.device == device else None
+        if live is not None or freeze is not None or rows is not None:
+            params = [t[0] for t in items]
+            if rows is not None and any(p.dim() == 0 or p.shape[0] != rows.numel() for p in params):
+                raise RuntimeError("FusedAdamW.set_grad_row_mask: every parameter must have one row per entry of the mask")
+            width = array.array("i", [p.numel() // p.shape[0] if p.dim() > 0 and p.shape[0] > 0 else 0 for p in params])
+            keep.append(width)
+            d.row_width = _at(width)
+            if live is not None:
+                d.live_rows = live.data_ptr()
+            if rows is not None:
+                d.grad_rows = rows.data_ptr()
+            if freeze is not None:
+                flags = array.array("i", [int(self.param_groups[t[3]].get("name") in freeze[1]) for t in items])
+                if any(fl and p.shape[0] > freeze[0].numel() for fl, p in zip(flags, params)):
+                    raise RuntimeError("FusedAdamW.set_row_freeze: the mask has fewer words than the tensor has rows")
+                if any(flags):
+                    keep.append(flags)
+                    d.row_freeze, d.group_frozen = freeze[0].data_ptr(), _at(flags)
+        return ctypes.addressof(d), keep

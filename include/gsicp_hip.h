@@ -406,6 +406,49 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
                            unsigned int* skipped_dev, const int* live_rows_dev, const int* row_width, const int* row_freeze_dev,
                            const int* group_frozen, const int* grad_rows_dev, void* stream);
 
+/* ---- AdamW over many tensors (no reference counterpart: the reference trains with torch.optim.Adam; these stand beside gsicp_adam_step) ----
+ * torch.optim.AdamW's step (amsgrad, maximize off) over any number of tensors, 40 per launch:
+ *     g' = *clip g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
+ *     p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
+ * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 is
+ * allowed, < 2^35), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap (checked; -2).
+ * clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's out + 1), or NULL.  step: the 1-based count after the increment.
+ * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (live_rows and the row masks: f32
+ * parameters of < 2^32 elements). */
+typedef struct {
+    const double* lr_dev;              /* DEVICE double[n] */
+    int* step_dev;                     /* DEVICE int: steps taken so far */
+    int bump_step;                     /* 0 leave the counter, 1 advance it after the update, 2 it has been advanced already */
+    const unsigned int* guard_count;   /* DEVICE or NULL: above guard_limit nothing moves and *skipped counts */
+    unsigned int guard_limit;
+    unsigned int* skipped;
+    const int* live_rows;              /* DEVICE int or NULL */
+    const int* row_width;              /* HOST int[n] or NULL */
+    const int* row_freeze;             /* DEVICE int[rows] or NULL */
+    const int* group_frozen;           /* HOST int[n] or NULL */
+    const int* grad_rows;              /* DEVICE int[rows] or NULL */
+} gsicp_adamw_device;
+int gsicp_adamw_step(int n, void* const* params, const void* const* grads, float* const* masters, float* const* exp_avg, float* const* exp_avg_sq,
+                     const long long* numel, const int* dtype, const double* lr, const double* weight_decay, double beta1, double beta2, double eps, int step,
+                     const float* clip, const gsicp_adamw_device* dev, void* stream);
+/* The same step with both moments in 8 bits: moments (uint16[numel]: low byte sign and 7-bit code of exp_avg, high byte code of exp_avg_sq) and block_exps
+ * (uint16[ceil(numel / 128)]: low / high byte the base exponent of the block's first / second moments).  A code c > 0 with base b is (1 + (c & 7) / 8) *
+ * 2^((c >> 3) + b - 127), 0 is zero; code 127 of the first moment is NaN, 255 of the second infinity.  All-zero arrays are the state before the first step.  Moments are
+ * rounded stochastically: with mix(x) = { x ^= x >> 16; x *= 0x7FEB352D; x ^= x >> 15; x *= 0x846CA68B; x ^= x >> 16 } and L = the eight odd words of lane_word (adamw.hip),
+ * element j of the tensor at place[k] (HOST int[n]; NULL: k) takes the halves of mix((j >> 3) ^ mix(seed + step * 0x9E3779B1 + place * 0x85EBCA6B)) * L[j & 7]: the same
+ * seed, step and place give the same bits.  The device form takes no live_rows and no row_freeze. */
+int gsicp_adamw_step_8bit(int n, void* const* params, const void* const* grads, float* const* masters, uint16_t* const* moments, uint16_t* const* block_exps,
+                          const long long* numel, const int* dtype, const double* lr, const double* weight_decay, double beta1, double beta2, double eps, int step,
+                          uint32_t seed, const int* place, const float* clip, const gsicp_adamw_device* dev, void* stream);
+/* Values of 8-bit moments, as f32 (dtype 0) or bf16 (1; exact). */
+int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* const* block_exps, void* const* exp_avg, void* const* exp_avg_sq, const long long* numel,
+                       int dtype, void* stream);
+/* out[0] = 2-norm over all elements of n tensors (dtype[k] as above; squares and sums in double, fixed order), out[1] = min(1, max_norm / (norm + 1e-6)) — the factor of
+ * torch.nn.utils.clip_grad_norm_ —, or 1 when max_norm <= 0.  out: DEVICE float[2]; scratch: DEVICE, gsicp_grad_norm_scratch_bytes(n), needs no initialisation. */
+size_t gsicp_grad_norm_scratch_bytes(int n);
+int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* out, void* scratch, void* stream);
+
 /* Map pruning without reallocation: GaussianModel.prune_points / _prune_optimizer
  * [REF scene/gaussian_model.py:409-447] apply one boolean mask to every parameter, both Adam moments and the per-Gaussian
  * statistics.  This moves the rows with keep[i] != 0 of `n_arrays` (<= 24) row-major DEVICE arrays from src[a] to dst[a] (distinct

@@ -1,0 +1,710 @@
+"""The AdamW step over many tensors (moments in 32 bits and in 8) and the global gradient norm, against a 64-bit restatement (oracle/adamw_oracle.py).
+
+Tolerances are the oracle's running bounds (each float32 operation and constant off by at most 2^-24 of its result), plus half a step of the output's type where it has 16 bits.
+8-bit moments are compared code by code: their float32 arithmetic is fixed operation by operation."""
+import numpy as np
+import pytest
+import torch
+
+from gs_icp_slam_amd import synth
+from oracle import adamw_oracle as ao
+from tests.util import make_settings, torch_inputs
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [0, 1, 2, 7, 8, 9, 16, 63, 127, 128, 129, 255, 256, 1000, 2047, 2048, 2049, 4096, 4097, 5003]
+MANY = (SIZES * 3)[:45]                       # more tensors than one launch takes
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+class Flat:
+    """Views of one buffer, each beginning wherever the last ended plus a gap of 1 to 5 elements; `intact()` says whether the gaps still hold what they held."""
+
+    def __init__(self, sizes, dtype, fill=7):
+        self.dtype, self.spans, at = dtype, [], 3
+        for i, n in enumerate(sizes):
+            self.spans.append((at, at + n))
+            at += n + 1 + i % 5
+        self.buf = torch.full((at + 8,), fill, dtype=dtype, device="cuda")
+        self.fill = fill
+        self.list = [self.buf[a:b] for a, b in self.spans]
+
+    def set(self, arrays):
+        for v, a in zip(self.list, arrays):
+            v.copy_(torch.as_tensor(a).to(self.dtype) if not torch.is_tensor(a) else a)
+        return self
+
+    def get(self):
+        host = self.buf.cpu()
+        return [host[a:b] for a, b in self.spans]
+
+    def intact(self):
+        gap = torch.ones(self.buf.numel(), dtype=torch.bool)
+        for a, b in self.spans:
+            gap[a:b] = False
+        return bool((self.buf.cpu()[gap] == self.fill).all())
+
+
+def _np(t):
+    return t.to(torch.float64).numpy()
+
+
+class Case:
+    """A set of tensors with their state on the device; `step()` makes one step and compares it with the oracle."""
+
+    def __init__(self, sizes, dtype, master, bits, seed=0, grad_scale=1e-3, eps=1e-15):
+        rng = np.random.default_rng(seed)
+        self.sizes, self.dtype, self.bits, self.eps, self.rng, self.grad_scale = sizes, dtype, bits, eps, rng, grad_scale
+        self.p = Flat(sizes, dtype).set([rng.normal(size=n).astype(np.float32) for n in sizes])
+        self.master = Flat(sizes, torch.float32).set([rng.normal(size=n).astype(np.float32) for n in sizes]) if master else None
+        self.g = Flat(sizes, dtype)
+        self.lr = [float(10.0 ** rng.uniform(-5, -1)) for _ in sizes]
+        self.wd = [float(rng.choice([0.0, 0.01, 0.3])) for _ in sizes]
+        m = [(rng.normal(size=n) * np.exp(2 * rng.normal(size=n)) * grad_scale * 0.3).astype(np.float32) for n in sizes]
+        v = [((rng.normal(size=n) * np.exp(2 * rng.normal(size=n)) * grad_scale) ** 2).astype(np.float32) for n in sizes]
+        if bits == 32:
+            self.s0, self.s1 = Flat(sizes, torch.float32).set(m), Flat(sizes, torch.float32).set(v)
+        else:
+            blocks = [-(-n // 128) for n in sizes]
+            enc = [ao.encode(a, b, *ao.random_bits(n, 1, 1, k)) for k, (a, b, n) in enumerate(zip(m, v, sizes))]
+            self.s0 = Flat(sizes, torch.int16).set([e[0].view(np.int16) for e in enc])
+            self.s1 = Flat(blocks, torch.int16).set([e[1].view(np.int16) for e in enc])
+
+    def step(self, t, betas=(0.9, 0.999), max_norm=None, seed=11):
+        from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit
+        rng = self.rng
+        self.g.set([(rng.normal(size=n) * np.exp(2 * rng.normal(size=n)) * self.grad_scale * (rng.random(n) < 0.7)).astype(np.float32) for n in self.sizes])
+        p0, g0, s0, s1 = self.p.get(), self.g.get(), self.s0.get(), self.s1.get()
+        w0 = self.master.get() if self.master else p0
+        kw = dict(lr=self.lr, step=t, betas=betas, eps=self.eps, weight_decay=self.wd, masters=self.master.list if self.master else None, max_norm=max_norm)
+        if self.bits == 32:
+            norm = adamw_step(self.p.list, self.g.list, self.s0.list, self.s1.list, **kw)
+        else:
+            norm = adamw_step_8bit(self.p.list, self.g.list, self.s0.list, self.s1.list, seed=seed, **kw)
+        clip = 1.0
+        if max_norm is not None:
+            want = np.float32(np.sqrt(sum((_np(g) ** 2).sum() for g in g0)))
+            assert norm.dtype == torch.float32 and abs(float(norm) - float(want)) <= 2.0 ** -23 * float(want)
+            clip = np.float32(min(1.0, max_norm / (float(norm) + 1e-6)))
+        p1, n0, n1 = self.p.get(), self.s0.get(), self.s1.get()
+        w1 = self.master.get() if self.master else None
+        for x in (self.p, self.g, self.s0, self.s1) + ((self.master,) if self.master else ()):
+            assert x.intact()
+        for k, n in enumerate(self.sizes):
+            if n == 0:
+                continue
+            g = _np(g0[k])
+            if self.bits == 32:
+                m, v = _np(s0[k]), _np(s1[k])
+            else:
+                m, v = ao.decode(s0[k].numpy(), s1[k].numpy())
+            (P, M, V), (dp, dm, dv) = ao.step64(_np(w0[k]), m, v, g, self.lr[k], self.wd[k], betas, self.eps, t, clip)
+            if self.bits == 32:
+                assert (np.abs(_np(n0[k]) - M) <= dm).all() and (np.abs(_np(n1[k]) - V) <= dv).all(), k
+            else:
+                m32, v32 = ao.step32(m, v, g, betas, None if max_norm is None else clip)
+                codes, exps = ao.encode(m32, v32, *ao.random_bits(n, seed, t, k))
+                assert np.array_equal(n0[k].numpy().view(np.uint16), codes) and np.array_equal(n1[k].numpy().view(np.uint16), exps), k
+            out = _np(p1[k])
+            if w1 is not None:
+                assert (np.abs(_np(w1[k]) - P) <= dp).all(), k
+                assert torch.equal(w1[k].to(self.dtype), p1[k]), k          # the parameter is the master, rounded once
+            else:
+                assert (np.abs(out - P) <= dp + HALF[self.dtype] * (np.abs(P) + dp) + TINY[self.dtype]).all(), (k, float(np.abs(out - P).max()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [("f32", False), ("bf16", False), ("bf16", True), ("f16", False), ("f16", True)])
+def test_steps_over_many_ragged_unaligned_tensors(bits, dtype, master):
+    c = Case(MANY, TYPES[dtype], master, bits, seed=bits, grad_scale=1e-2 if dtype == "f16" else 1e-3)
+    for t in (1, 2, 1000):
+        c.step(t)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [1e-3, 1e6])
+def test_clipping_inside_the_step(bits, max_norm):
+    c = Case(MANY, torch.float32, False, bits, seed=3)
+    for t in (5, 6):
+        c.step(t, max_norm=max_norm)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("betas,eps", [((0.0, 0.0), 1e-8), ((0.95, 0.99999), 1e-3), ((0.5, 0.9), 0.5)])
+def test_other_betas_and_eps(bits, betas, eps):
+    Case([300, 5, 4100], torch.float32, False, bits, seed=9, eps=eps).step(3, betas=betas)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_large_tensor_beside_small_ones_over_many_workgroups(bits):
+    Case([9, 5_000_011, 1, 700], torch.float32, False, bits, seed=2).step(50)
+
+
+def test_wide_range_inside_a_block_of_8_bit_moments():
+    """Blocks whose values span far more than the codes' exponents, values at the ends of float32, subnormals, zeros of both signs."""
+    from gs_icp_slam_amd.optim import adamw_step_8bit
+    n = 1024
+    g = np.zeros(n, dtype=np.float32)
+    g[:128] = 10.0 ** np.linspace(-20, 5, 128)
+    g[128:256] = -1e-18 * np.arange(128)                 # squares are subnormal or vanish
+    g[256:384] = 1e19                                    # squares near the largest float
+    g[384:512] = np.float32(1e-42)                       # subnormal gradients
+    g[512:640] = -0.0
+    g[640] = 3e38                                        # its square is infinite, the gradient is not
+    p, gd = torch.ones(n, device="cuda"), torch.from_numpy(g).cuda()
+    mo, be = torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(n // 128, dtype=torch.int16, device="cuda")
+    m, v = np.zeros(n, dtype=np.float32), np.zeros(n, dtype=np.float32)
+    for t in (1, 2, 3):
+        adamw_step_8bit([p], [gd], [mo], [be], lr=1e-3, step=t, seed=4)
+        m32, v32 = ao.step32(m, v, g, (0.9, 0.999))
+        codes, exps = ao.encode(m32, v32, *ao.random_bits(n, 4, t, 0))
+        assert np.array_equal(mo.cpu().numpy().view(np.uint16), codes) and np.array_equal(be.cpu().numpy().view(np.uint16), exps), t
+        m, v = ao.decode(codes, exps, np.float32)
+    assert bool(torch.isfinite(p).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_values_that_are_not_finite_stay_in_their_element(bits):
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, decode_moments
+    n = 4000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    g = torch.randn(n, device="cuda", generator=gen)
+    bad = {5: float("nan"), 130: float("inf"), 131: float("-inf"), 3999: float("nan")}
+    runs = []
+    for spoil in (False, True):
+        gg = g.clone()
+        if spoil:
+            for i, x in bad.items():
+                gg[i] = x
+        else:
+            for i in bad:
+                gg[i] = 0.0
+        p = torch.ones(n, device="cuda")
+        for t in (1, 2):
+            if bits == 32:
+                if t == 1:
+                    s = [torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")]
+                adamw_step([p], [gg], [s[0]], [s[1]], lr=1e-2, step=t)
+            else:
+                if t == 1:
+                    s = [torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(32, dtype=torch.int16, device="cuda")]
+                adamw_step_8bit([p], [gg], [s[0]], [s[1]], lr=1e-2, step=t)
+        m, v = (s if bits == 32 else [x[0] for x in decode_moments([s[0]], [s[1]])])
+        runs.append((p.cpu(), m.cpu(), v.cpu()))
+    hit = torch.zeros(n, dtype=torch.bool)
+    hit[list(bad)] = True
+    (p0, m0, v0), (p1, m1, v1) = runs
+    for a, b in ((p0, p1), (m0, m1), (v0, v1)):
+        assert torch.equal(a[~hit], b[~hit])
+    assert not torch.isfinite(p1[hit]).any() and not torch.isfinite(m1[hit]).any() and not torch.isfinite(v1[hit]).any()
+
+
+def test_same_call_same_bits_and_other_seed_other_bits():
+    from gs_icp_slam_amd.optim import adamw_step_8bit
+    n = 100_000
+    g = torch.randn(n, device="cuda")
+    outs = []
+    for seed in (1, 1, 2, 1 + (1 << 32)):
+        p, mo, be = torch.zeros(n, device="cuda"), torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(782, dtype=torch.int16, device="cuda")
+        adamw_step_8bit([p], [g], [mo], [be], lr=0.1, step=1, seed=seed)
+        outs.append(mo)
+    assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], outs[2]) and torch.equal(outs[0], outs[3])     # a seed has 32 bits
+
+
+# ------------------------------------------------------------------------------------------------ values of the codes
+def test_decode_of_every_code_with_every_kind_of_base():
+    from gs_icp_slam_amd.optim import decode_moments
+    every = np.arange(65536, dtype=np.uint16)
+    bases = [(1, 1), (1, 224), (240, 1), (113, 97), (240, 224), (0, 0)]
+    codes = np.concatenate([every] * len(bases))
+    exps = np.concatenate([np.full(512, bm | bv << 8, dtype=np.uint16) for bm, bv in bases])
+    c, e = (torch.from_numpy(x.view(np.int16).copy()).cuda() for x in (codes, exps))
+    used = np.ones(codes.size, dtype=bool)
+    used[-65536:] = every == 0                            # base 0 is the state before the first step: zeros only
+    used &= ((codes & 127) <= 120) | ((codes & 127) == 127)      # a base leaves room up to its block's largest value and a carry
+    used &= ((codes >> 8) <= 248) | ((codes >> 8) == 255)
+    m, v = ao.decode(codes, exps)
+    for dtype in (torch.float32, torch.bfloat16):
+        (gm,), (gv,) = decode_moments([c], [e], dtype=dtype)
+        assert gm.dtype == gv.dtype == dtype
+        gm, gv = _np(gm.cpu()), _np(gv.cpu())
+        with np.errstate(over="ignore"):
+            wm, wv = m.astype(np.float32).astype(np.float64), v.astype(np.float32).astype(np.float64)
+        fits = used & (np.isnan(m) | (np.abs(m) < 2.0 ** 128)) & (np.isinf(v) | (v < 2.0 ** 128))
+        assert fits.sum() > 0.8 * used.sum()
+        np.testing.assert_array_equal(gm[fits], wm[fits])
+        np.testing.assert_array_equal(gv[fits], wv[fits])
+
+
+def test_decode_keeps_shapes_over_many_tensors():
+    from gs_icp_slam_amd.optim import decode_moments, new_moments_8bit
+    ps = [torch.empty(s, device="cuda") for s in [(3, 5), (0, 4), (), (1000,), (129, 2)] * 14]
+    st = [new_moments_8bit(p) for p in ps]
+    for c, e in st:
+        c.random_(0, 120)
+        e.fill_(100 | 90 << 8)
+    ms, vs = decode_moments([s[0] for s in st], [s[1] for s in st])
+    for p, (c, e), m, v in zip(ps, st, ms, vs):
+        wm, wv = ao.decode(c.cpu().numpy().reshape(-1), e.cpu().numpy())
+        assert m.shape == v.shape == p.shape and np.array_equal(_np(m.cpu()).reshape(-1), wm) and np.array_equal(_np(v.cpu()).reshape(-1), wv)
+    assert decode_moments([], []) == ([], [])
+
+
+# ------------------------------------------------------------------------------------------------ global norm
+@pytest.mark.parametrize("sizes", [[1], [0], [0, 0, 3], MANY, [7, 12] * 100, [3_000_001, 5]])
+def test_grad_norm_over_mixed_types(sizes):
+    from gs_icp_slam_amd.optim import grad_norm
+    rng = np.random.default_rng(len(sizes))
+    flats = [Flat(sizes[i::3], dt).set([rng.normal(size=n) for n in sizes[i::3]]) for i, dt in enumerate(TYPES.values())]
+    ts = [t for f in flats for t in f.list]
+    want = np.sqrt(sum(float((t.double() ** 2).sum()) for t in ts))
+    got = grad_norm(ts)
+    assert got.shape == () and got.dtype == torch.float32
+    assert abs(float(got) - want) <= 2.0 ** -24 * 1.0001 * want           # rounded once
+    assert torch.equal(got, grad_norm(ts))
+
+
+@pytest.mark.parametrize("dtype", TYPES.values())
+def test_grad_norm_of_extremes(dtype):
+    from gs_icp_slam_amd.optim import grad_norm
+    top = torch.finfo(dtype).max
+    for x in (top / 256, torch.finfo(dtype).tiny, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps):
+        t = torch.full((100,), x, dtype=dtype, device="cuda")
+        want = 10.0 * float(t[0].double())
+        assert abs(float(grad_norm([t])) - want) <= 2.0 ** -24 * want + 2.0 ** -150, (dtype, x)       # no overflow or underflow of the squares
+    t = torch.zeros(5000, dtype=dtype, device="cuda")
+    assert float(grad_norm([t])) == 0.0
+    t[4999] = float("inf")
+    assert float(grad_norm([t])) == float("inf")
+    t[3] = float("nan")
+    assert np.isnan(float(grad_norm([t])))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_norm_that_is_not_finite_clips_like_torch(bits):
+    """clip_grad_norm_'s factor of an infinite norm is 0, of NaN it is NaN."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    for bad, finite in ((float("inf"), True), (float("nan"), False)):
+        p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+        opt = FusedAdamW([p], lr=0.1, weight_decay=0.0, max_grad_norm=1.0, state_bits=bits)
+        p.grad = torch.ones_like(p)
+        p.grad[3] = bad
+        opt.step()
+        ok = torch.isfinite(p.detach())
+        assert ok.tolist() == [finite and i != 3 for i in range(10)]          # inf * 0 is NaN in its own element, as in torch
+
+
+# ------------------------------------------------------------------------------------------------ positions past 32 bits
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_past_two_to_the_32(bits):
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, grad_norm
+    n = (1 << 32) + 2048 + 77
+    rng = np.random.default_rng(0)
+    windows = [(0, 640), ((1 << 31) - 256, (1 << 31) + 256), ((1 << 32) - 256, (1 << 32) + 256), (n - 77 - 128, n)]
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    for a, b in windows:
+        p[a:b] = torch.from_numpy(rng.normal(size=b - a)).cuda().bfloat16()
+        g[a:b] = torch.from_numpy(rng.normal(size=b - a)).cuda().bfloat16()
+    before = [(_np(p[a:b].cpu()), _np(g[a:b].cpu())) for a, b in windows]
+    want = np.sqrt(sum((x[1] ** 2).sum() for x in before))
+    assert abs(float(grad_norm([g])) - want) <= 2.0 ** -23 * want
+    if bits == 32:
+        s = [torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")]
+        adamw_step([p], [g], [s[0]], [s[1]], lr=1e-2, step=1)
+    else:
+        s = [torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(-(-n // 128), dtype=torch.int16, device="cuda")]
+        adamw_step_8bit([p], [g], [s[0]], [s[1]], lr=1e-2, step=1, seed=5)
+    for (a, b), (p0, g0) in zip(windows, before):
+        zero = np.zeros(b - a)
+        (P, M, V), (dp, dm, dv) = ao.step64(p0, zero, zero, g0, 1e-2, 1e-2, (0.9, 0.999), 1e-8, 1)
+        assert (np.abs(_np(p[a:b].cpu()) - P) <= dp + 2.0 ** -8 * (np.abs(P) + dp)).all(), a
+        if bits == 32:
+            assert (np.abs(_np(s[0][a:b].cpu()) - M) <= dm).all() and (np.abs(_np(s[1][a:b].cpu()) - V) <= dv).all(), a
+        else:
+            codes, exps = ao.encode(*ao.step32(zero, zero, g0, (0.9, 0.999)), *ao.random_bits(b - a, 5, 1, 0, first=a))
+            assert np.array_equal(s[0][a:b].cpu().numpy().view(np.uint16), codes), a
+            assert np.array_equal(s[1][a // 128: -(-b // 128)].cpu().numpy().view(np.uint16), exps), a
+    inside = sum(int((p[a:b] != 0).sum()) for a, b in windows)
+    total = sum(int((c != 0).sum()) for c in p.split(1 << 28))
+    assert inside == total                                                   # nothing moved elsewhere
+
+
+# ------------------------------------------------------------------------------------------------ the optimiser
+def _params(seed=0, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(s, generator=gen).to(dtype).cuda()) for s in [(300, 3), (300, 1, 3), (300, 0, 3), (300, 1), (17,), (), (65, 33)]]
+
+
+def _feed(params, seed):
+    gen = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.shape, generator=gen) * 0.1).to(p.dtype).cuda()
+
+
+def test_optimiser_follows_torch_adamw_over_groups():
+    from gs_icp_slam_amd.optim import FusedAdamW
+    ours = _params()
+    theirs = [torch.nn.Parameter(p.detach().cpu().double()) for p in ours]
+    groups = lambda ps: [{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:5], "lr": 3e-3, "weight_decay": 0.3}, {"params": ps[5:], "betas": (0.8, 0.99), "eps": 1e-6}]   # noqa: E731
+    a = FusedAdamW(groups(ours), lr=1e-3, weight_decay=0.05, max_grad_norm=0.7)
+    b = torch.optim.AdamW(groups(theirs), lr=1e-3, weight_decay=0.05)
+    steps = 12
+    for k in range(steps):
+        _feed(ours, k)
+        for p, q in zip(ours, theirs):
+            q.grad = p.grad.cpu().double()
+        if k == 4:
+            ours[1].grad, theirs[1].grad = None, None                          # its step count falls behind the others'
+        if k == 6:
+            a.param_groups[0]["lr"] = b.param_groups[0]["lr"] = 2e-2
+        norm = torch.nn.utils.clip_grad_norm_(theirs, 0.7)
+        a.step()
+        b.step()
+        assert abs(float(a.last_grad_norm) - float(norm)) <= 2.0 ** -23 * float(norm)
+    for p, q, in zip(ours, theirs):
+        # a step is off by the roundings of the parameter (3 of 2^-24) and of an update of at most lr * 10 (some 20 of them, with the moments' own)
+        assert (p.detach().cpu().double() - q.detach()).abs().max() <= steps * 2.0 ** -24 * (3 * 4 + 40 * 2e-2 * 10) if p.numel() else True
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_state_dict_round_trip_continues_bit_for_bit(bits, dtype, tmp_path):
+    from gs_icp_slam_amd.optim import FusedAdamW
+    kw = dict(lr=1e-2, state_bits=bits, master_weights=True, seed=77)
+    a_params = _params(1, dtype)
+    a = FusedAdamW(a_params, **kw)
+    for k in range(3):
+        _feed(a_params, k)
+        a.step()
+    torch.save(a.state_dict(), tmp_path / "s.pt")
+    b_params = [torch.nn.Parameter(p.detach().clone()) for p in a_params]
+    b = FusedAdamW(b_params, **kw)
+    b.load_state_dict(torch.load(tmp_path / "s.pt", weights_only=True))
+    for k in range(3, 6):
+        for ps, o in ((a_params, a), (b_params, b)):
+            _feed(ps, k)
+            o.step()
+    for p, q in zip(a_params, b_params):
+        assert torch.equal(p, q)
+        for name in a.state[p]:
+            x, y = a.state[p][name], b.state[q][name]
+            assert (torch.equal(x, y) and x.dtype == y.dtype) if torch.is_tensor(x) else x == y, name
+        if dtype != torch.float32:
+            assert a.state[p]["master"].dtype == torch.float32
+    m, v = a.moments(a_params[0])
+    assert m.dtype == v.dtype == torch.float32 and m.shape == a_params[0].shape and bool((v > 0).all())
+
+
+def test_places_of_parameters_do_not_depend_on_which_have_gradients():
+    from gs_icp_slam_amd.optim import FusedAdamW
+    full, part = _params(2), _params(2)
+    a, b = FusedAdamW(full, state_bits=8), FusedAdamW(part, state_bits=8)
+    _feed(full, 0)
+    _feed(part, 0)
+    part[0].grad = part[3].grad = None
+    a.step()
+    b.step()
+    for i in (1, 4, 6):
+        assert torch.equal(full[i], part[i]) and torch.equal(a.state[full[i]]["moments"], b.state[part[i]]["moments"])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_captured_steps_follow_eager_ones(bits, max_norm):
+    """Two graphs of one capturable optimiser, replayed in turn with eager steps, other work and synchronisations between, against the host form."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    host, dev = _params(3), _params(3)
+    kw = dict(lr=1e-2, weight_decay=0.1, state_bits=bits, max_grad_norm=max_norm, seed=5)
+    a, b = FusedAdamW(host, **kw), FusedAdamW(dev, capturable=True, **kw)
+    steps = 0
+
+    def eager_pair(k, graph=None):
+        nonlocal steps
+        _feed(host, k)
+        a.step()
+        if graph is None:
+            _feed(dev, k)
+            b.step()
+        else:
+            for p, q in zip(host, static):
+                q.copy_(p.grad)
+            graph.replay()
+        steps += 1
+        for p, q in zip(host, dev):
+            if p.numel() == 0:
+                continue
+            sa, sb = a.state[p], b.state[q]
+            for name in ("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps"):
+                assert torch.equal(sa[name], sb[name]), (k, name)
+            # the bias corrections come from another pow(): step size and root within 2^-23 of each other, rounding per step
+            assert (p - q).abs().max() <= steps * 2.0 ** -23 * (4 + 10 * 1e-2 * 4), k
+        assert int(b.state[dev[0]]["step"]) == steps == a.state[host[0]]["step"]
+        if max_norm is not None and graph is None:
+            assert torch.equal(a.last_grad_norm, b.last_grad_norm)
+
+    for k in range(2):
+        eager_pair(k)
+    static = [torch.zeros_like(p) for p in dev]
+    graphs = []
+    for _ in range(2):
+        for p, q in zip(dev, static):
+            p.grad = q
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            b.step()
+        graphs.append(g)
+    assert int(b.state[dev[0]]["step"]) == 2                          # capturing executes nothing
+    for k, which in enumerate([0, 1, 1, 0, None, 0, 1]):
+        torch.randn(1 << 20, device="cuda").sum().item()              # other eager work, with a synchronisation
+        eager_pair(10 + k, None if which is None else graphs[which])
+    b.param_groups[0]["lr"] = a.param_groups[0]["lr"] = 2e-2          # a new learning rate reaches the replays
+    b.sync_lr()
+    eager_pair(30, graphs[0])
+
+
+def test_steps_on_another_stream():
+    from gs_icp_slam_amd.optim import FusedAdamW
+    one, two = _params(4), _params(4)
+    a, b = FusedAdamW(one, max_grad_norm=0.1, state_bits=8), FusedAdamW(two, max_grad_norm=0.1, state_bits=8)
+    side = torch.cuda.Stream()
+    for k in range(4):
+        _feed(one, k)
+        a.step()
+        _feed(two, k)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            b.step()
+        torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for p, q in zip(one, two):
+        assert torch.equal(p, q)
+
+
+# ------------------------------------------------------------------------------------------------ the map
+NAMES = ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")
+LRS = {"xyz": 4e-6, "f_dc": 2.5e-3, "f_rest": 1.25e-4, "opacity": 0.05, "scaling": 5e-3, "rotation": 1e-3}
+
+
+def _rows(k, n_rest, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen)      # noqa: E731
+    return {"xyz": r(k, 3), "f_dc": r(k, 1, 3), "f_rest": r(k, n_rest, 3), "opacity": r(k, 1), "scaling": r(k, 3), "rotation": r(k, 4)}
+
+
+@pytest.mark.parametrize("stable", [False, True])
+@pytest.mark.parametrize("n_rest", [0, 15])
+def test_a_map_that_grows_and_is_pruned(stable, n_rest):
+    """GaussianStore with FusedAdamW against the same rows kept as plain tensors, concatenated and indexed by hand."""
+    from gs_icp_slam_amd.gaussian_store import GaussianStore
+    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step
+    store = GaussianStore(4000, n_rest=n_rest, stable=stable)
+    first = _rows(1500, n_rest, 0)
+    store.append(first)
+    opt = store.attach(FusedAdamW, LRS, lr=0.0, eps=1e-15, weight_decay=0.02, capturable=stable)
+    p = {k: first[k].clone() for k in NAMES}
+    m, v = ({k: torch.zeros_like(p[k]) for k in NAMES} for _ in range(2))
+    t = 0
+    for op in ("step", "step", "grow", "step", "prune", "step", "grow", "step"):
+        if op == "grow":
+            new = _rows(700, n_rest, 100 + t)
+            store.append(new)
+            for k in NAMES:
+                p[k] = torch.cat((p[k], new[k]))
+                m[k], v[k] = (torch.cat((x[k], torch.zeros_like(new[k]))) for x in (m, v))
+        elif op == "prune":
+            remove = torch.rand(store.n, device="cuda") < 0.3
+            store.prune(remove)
+            p, m, v = ({k: x[k][~remove].contiguous() for k in NAMES} for x in (p, m, v))
+        else:
+            t += 1
+            grads = {k: g * 0.1 for k, g in _rows(store.n, n_rest, 50 + t).items()}
+            for k in NAMES:
+                full = torch.full_like(store.params[k], float("nan")) if stable else grads[k].clone()      # rows behind the live count are not read
+                full[: store.n] = grads[k]
+                store.params[k].grad = full
+            opt.step()
+            adamw_step([p[k] for k in NAMES], [grads[k] for k in NAMES], [m[k] for k in NAMES], [v[k] for k in NAMES], lr=[LRS[k] for k in NAMES], step=t, eps=1e-15,
+                       weight_decay=0.02)
+        assert store.n == p["xyz"].shape[0]
+        for k in NAMES:
+            assert torch.equal(store.view("m", k), m[k]) and torch.equal(store.view("v", k), v[k]), (op, k)
+            if stable:        # the device form takes its bias corrections from another pow()
+                assert p[k].numel() == 0 or (store.live(k) - p[k]).abs().max() <= t * 2.0 ** -22 * (5 + 10 * LRS[k]), (op, k)
+            else:
+                assert torch.equal(store.live(k), p[k]), (op, k)
+    if stable:
+        assert all(not bool(store.view("p", k).isnan().any()) and not bool(store.params[k].isnan().any()) for k in NAMES)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_row_masks_and_guard_equal_a_step_on_masked_gradients(bits):
+    """Culled rows count as zero gradients whatever the memory holds; frozen rows (32-bit moments) do not move; a tripped guard moves nothing."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    rows = 2777
+    shapes = [(rows, 3), (rows, 1, 3), (rows, 15, 3), (rows, 1), (rows, 4), (rows, 7)]
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    ps = [torch.randn(s, device="cuda", generator=gen) for s in shapes]
+    make = lambda: [torch.nn.Parameter(p.clone()) for p in ps]       # noqa: E731
+    a_p, b_p = make(), make()
+    groups = lambda q: [{"params": [p], "name": str(i)} for i, p in enumerate(q)]    # noqa: E731
+    a, b = (FusedAdamW(groups(q), lr=1e-2, capturable=True, state_bits=bits, seed=3) for q in (a_p, b_p))
+    guard = torch.zeros(1, dtype=torch.int32, device="cuda")
+    b.set_overflow_guard(guard, 10)
+    frozen = (torch.rand(rows, device="cuda", generator=gen) < 0.3).to(torch.int32)
+    if bits == 32:
+        b.set_row_freeze(frozen, ("0", "2"))
+    for k in range(4):
+        radii = torch.randint(-1, 3, (rows,), dtype=torch.int32, device="cuda", generator=gen)
+        for p, q in zip(a_p, b_p):
+            g = torch.randn(p.shape, device="cuda", generator=gen)
+            q.grad = g.clone()
+            q.grad[radii <= 0] = float("nan")
+            g[radii <= 0] = 0.0
+            p.grad = g
+        b.set_grad_row_mask(radii)
+        if k == 2:
+            guard.fill_(11)
+            before = [q.detach().clone() for q in b_p]
+            b.step()
+            assert all(torch.equal(x, q) for x, q in zip(before, b_p)) and int(b.skipped_steps) == 1
+            guard.zero_()
+        keep = [(p.detach().clone(), {n: s.clone() for n, s in a.state[p].items()} if a.state[p] else None) for p in a_p]
+        a.step()
+        b.step()
+        for i, (p, q) in enumerate(zip(a_p, b_p)):
+            if bits == 32 and i in (0, 2):      # undo the twin's frozen rows: they were no parameters
+                fz = frozen.bool()
+                with torch.no_grad():
+                    p[fz] = keep[i][0][fz]
+                    for n in ("exp_avg", "exp_avg_sq"):
+                        a.state[p][n][fz] = keep[i][1][n][fz] if keep[i][1] else 0.0
+            assert torch.equal(p, q), (k, i)
+            for n in a.state[p]:
+                assert torch.equal(a.state[p][n], b.state[q][n]), (k, i, n)
+    assert int(b.state[b_p[0]]["step"]) == 4
+
+
+@pytest.mark.parametrize("bits,max_norm", [(32, None), (8, None), (32, 1e-3), (8, 1e-3)])
+def test_captured_mapper_iteration_takes_it(bits, max_norm, monkeypatch):
+    """The mapper iteration as one graph (sparse gradient rows, the step bump inside the loss kernel) with FusedAdamW, against the same with both switched off."""
+    from diff_gaussian_rasterization import GaussianRasterizer
+    from gs_icp_slam_amd.graph import MapperIterationGraph
+    from gs_icp_slam_amd.optim import FusedAdamW
+    P, W, H = 20000, 320, 200
+    cfg = dict(synth.REPLICA)
+    cam = synth.make_camera(W, H, cfg["fx"] * W / cfg["W"], cfg["fy"] * H / cfg["H"], synth.DEFAULT_POSE_A)
+    g = synth.s_map(P, seed=5)
+    raw = {"means3D": torch.from_numpy(g["means3D"]), "scales": torch.log(torch.from_numpy(g["scales"])), "rotations": torch.from_numpy(g["rotations"]),
+           "opacities": torch.logit(torch.from_numpy(g["opacities"]).clamp(1e-4, 1 - 1e-4)), "shs": torch.from_numpy(g["shs"])}
+    lrs = {"means3D": 4e-6, "shs": 2.5e-3, "opacities": 0.05, "scales": 5e-3, "rotations": 1e-3}
+    rs = make_settings(cam, [0.0, 0.0, 0.0])
+    t2 = torch_inputs(synth.s_map(P, seed=5, perturb_seed=7))
+    with torch.no_grad():
+        depth, color, _, _ = GaussianRasterizer(rs)(means3D=t2["means3D"], means2D=torch.zeros_like(t2["means3D"]), shs=t2["shs"], opacities=t2["opacities"],
+                                                    scales=t2["scales"], rotations=t2["rotations"])
+    res = []
+    for fast in (True, False):
+        for k in ("GSICP_SPARSE_GRADS", "GSICP_STEP_BUMP_IN_LOSS"):
+            monkeypatch.setenv(k, "1" if fast else "0")
+        params = {k: v.cuda().contiguous().requires_grad_(True) for k, v in raw.items()}
+        opt = FusedAdamW([{"params": [params[k]], "lr": lr} for k, lr in lrs.items()], lr=0.0, eps=1e-15, weight_decay=1e-3, capturable=True, state_bits=bits,
+                         max_grad_norm=max_norm, seed=9)
+        mg = MapperIterationGraph(params, opt, H, W, cam["tanfovx"], cam["tanfovy"], sh_degree=0, capacity=2_000_000, warmup=2)
+        assert mg._sparse == (fast and max_norm is None)
+        mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+        start = {k: v.detach().clone() for k, v in params.items()}
+        mg.capture()
+        assert all(torch.equal(start[k], params[k]) for k in params)
+        losses = []
+        for k in range(5):
+            mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+            losses.append(float(mg.step()))
+            torch.cuda.synchronize()
+        assert not mg.overflowed() and all(np.isfinite(losses))
+        assert all(not torch.equal(start[k], params[k]) for k in params)
+        res.append((losses, [v.detach().clone() for v in params.values()], [{n: s.clone() for n, s in opt.state[v].items()} for v in params.values()]))
+        assert int(opt.state[params["means3D"]]["step"]) == 5
+        mg.release()
+    assert res[0][0] == res[1][0]
+    for a, b in zip(res[0][1], res[1][1]):
+        assert torch.equal(a, b)
+    for a, b in zip(res[0][2], res[1][2]):
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_a_run_of_the_operators_together():
+    """Norm, 8-bit step, decode, 32-bit step from the decoded moments: as a program uses them that moves from 8-bit to 32-bit moments."""
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, decode_moments, grad_norm, new_moments_8bit
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    ps = [torch.randn(s, device="cuda", generator=gen) for s in [(1000, 3), (1000, 15, 3), (1000, 1), (64, 7)]]
+    st = [new_moments_8bit(p) for p in ps]
+    for t in range(1, 5):
+        gs = [torch.randn(p.shape, device="cuda", generator=gen) for p in ps]
+        want = np.sqrt(sum(float((g.double() ** 2).sum()) for g in gs))
+        norm = grad_norm(gs)
+        got = adamw_step_8bit(ps, gs, [s[0] for s in st], [s[1] for s in st], lr=1e-2, step=t, seed=2, max_norm=1.0)
+        assert torch.equal(norm, got) and abs(float(norm) - want) <= 2.0 ** -23 * want
+    m, v = decode_moments([s[0] for s in st], [s[1] for s in st])
+    before = [(_np(p.cpu()).reshape(-1), _np(a.cpu()).reshape(-1), _np(b.cpu()).reshape(-1)) for p, a, b in zip(ps, m, v)]
+    gs = [torch.randn(p.shape, device="cuda", generator=gen) for p in ps]
+    adamw_step(ps, gs, m, v, lr=1e-2, step=5)
+    for p, g, (p0, m0, v0), a, b in zip(ps, gs, before, m, v):
+        (P, M, V), (dp, dm, dv) = ao.step64(p0, m0, v0, _np(g.cpu()).reshape(-1), 1e-2, 1e-2, (0.9, 0.999), 1e-8, 5)
+        for x, y, d in ((p, P, dp), (a, M, dm), (b, V, dv)):
+            assert (np.abs(_np(x.cpu()).reshape(-1) - y) <= d).all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals that need a device
+def test_refusals_on_the_device():
+    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step, adamw_step_8bit, decode_moments, grad_norm
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")        # noqa: E731
+    ok = dict(lr=1e-3, step=1)
+    buf = z(100)
+    same = z(8)
+    bad = [
+        lambda: adamw_step([same, same], [z(8), z(8)], [z(8), z(8)], [z(8), z(8)], **ok),             # one tensor twice
+        lambda: adamw_step([buf[:60], buf[50:]], [z(60), z(50)], [z(60), z(50)], [z(60), z(50)], **ok),
+        lambda: adamw_step([z(8)], [z(8)], [same], [same], **ok),
+        lambda: adamw_step([z(8)], [z(9)], [z(8)], [z(8)], **ok),
+        lambda: adamw_step([z(8)], [z(8, dt=torch.bfloat16)], [z(8)], [z(8)], **ok),
+        lambda: adamw_step([z(8)], [z(8)], [z(8, dt=torch.bfloat16)], [z(8)], **ok),
+        lambda: adamw_step([z(8, dt=torch.float64)], [z(8, dt=torch.float64)], [z(8)], [z(8)], **ok),
+        lambda: adamw_step([z(8, 4).t()], [z(4, 8)], [z(4, 8)], [z(4, 8)], **ok),
+        lambda: adamw_step([z(8)], [z(8, 2)[:, 0]], [z(8)], [z(8)], **ok),
+        lambda: adamw_step([z(8)], [z(8).cpu()], [z(8)], [z(8)], **ok),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [], **ok),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], lr=[1e-3, 1e-3], step=1),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], lr=1e-3, step=0),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], betas=(1.0, 0.9), **ok),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], max_norm=0.0, **ok),
+        lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], masters=[z(8)], **ok),                     # an f32 parameter has no master
+        lambda: adamw_step_8bit([z(200)], [z(200)], [z(200, dt=torch.int16)], [z(1, dt=torch.int16)], **ok),
+        lambda: adamw_step_8bit([z(200)], [z(200)], [z(200)], [z(2, dt=torch.int16)], **ok),
+        lambda: decode_moments([z(200, dt=torch.int16)], [z(2, dt=torch.int16)], dtype=torch.float16),
+        lambda: grad_norm([]),
+        lambda: grad_norm([z(4, dt=torch.int32)]),
+    ]
+    for k, f in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            f()
+            pytest.fail(f"call {k} was not refused")
+    assert adamw_step([], [], [], [], **ok) is None
+    opt = FusedAdamW([torch.nn.Parameter(z(8))], state_bits=8, capturable=True)
+    with pytest.raises(RuntimeError):
+        opt.set_live_rows(z(1, dt=torch.int32))
+    with pytest.raises(RuntimeError):
+        opt.set_row_freeze(z(8, dt=torch.int32), ("x",))
+    p = torch.nn.Parameter(z(8, 2))
+    opt = FusedAdamW([p], capturable=True, max_grad_norm=1.0)
+    p.grad = z(8, 2)
+    opt.set_grad_row_mask(z(8, dt=torch.int32))
+    with pytest.raises(RuntimeError):
+        opt.step()
+    opt.set_grad_row_mask(None)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(g):       # the learning rates have no device copy yet
+            opt.step()

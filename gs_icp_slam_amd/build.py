@@ -80,10 +80,30 @@ def build(force=False, verbose=True):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    build_tensor_lists(force=force, verbose=verbose)
     build_experiments(force=force, verbose=verbose)
     build_pybind_module(force=force, verbose=verbose)
     build_torch_ext_module(force=force, verbose=verbose)
     return OUT
+
+
+def build_tensor_lists(force=False, verbose=True):
+    """csrc/tensor_lists.cpp -> gs_icp_slam_amd/_tensor_lists.<abi>.so: lists of torch tensors as host arrays of the C ABI (the many-tensor operators of optim.py).  Plain g++
+    against libtorch's headers: host code only."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "tensor_lists.cpp")
+    out = os.path.join(HERE, "_tensor_lists" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+    if force or _newer(out, [src]):
+        tl = _torch_lib_dir()
+        cmd = (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wno-deprecated-declarations", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{p}" for p in cpp_extension.include_paths()] +
+               [f"-I{sysconfig.get_paths()['include']}", src, "-o", out, f"-L{tl}", f"-Wl,-rpath,{tl}", "-lc10", "-ltorch_cpu", "-ltorch_python"])
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+    return out
 
 
 def build_pybind_module(force=False, verbose=True):

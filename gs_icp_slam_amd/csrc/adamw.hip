@@ -41,7 +41,8 @@ constexpr int TABLE = 40;             // tensors per launch: the table travels i
 constexpr int NORM_TABLE = 64;
 constexpr int TILE_ELEMS = 2048;      // elements per workgroup and pass: 256 lanes x 8
 constexpr int STEP_GRID = 2048;       // workgroups of a large launch (8 per CU)
-constexpr int NORM_GRID = 1024;       // partial sums of one norm launch
+constexpr int NORM_GRID = 2048;       // partial sums of one norm launch
+constexpr int NORM_SMALL_TILES = 128; // 4 KB tiles that one workgroup of 16 waves takes by itself
 constexpr int QBLOCK = 128;           // elements per base exponent: 16 lanes x 8
 
 enum Dtype { F32 = 0, BF16 = 1, F16 = 2 };
@@ -396,54 +397,98 @@ __global__ __launch_bounds__(256) void adamw_decode_kernel(DecodeTable t, uint32
 }
 
 // ------------------------------------------------------------------------------------------------ global norm
+// Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split, and the squares of large
+// or small f32 gradients would leave its range.  The sums are split over the workgroups by position alone and joined in a fixed order.
 struct NormEntry { const void* g; long long numel; int dtype, pad; };
 struct NormTable { uint32_t first[64]; NormEntry e[NORM_TABLE]; };
 
-template <int DT, bool FULL>
-__device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile) {
-    const long long at = (long long)tile * TILE_ELEMS + 8 * threadIdx.x;
-    const int nv = FULL ? 8 : (int)max(0ll, min(8ll, e.numel - at));
-    float g[8];
-    load8<DT, FULL>(e.g, at, nv, g);
+__host__ __device__ constexpr int norm_tile_elems(int dtype, int bytes) { return bytes / (dtype == F32 ? 4 : 2); }
+
+template <int DT>
+__device__ __forceinline__ double square_sum16(const u32x4& r) {      // of one 16-byte load
     double s = 0.0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = __builtin_fma((double)g[j], (double)g[j], s);
+    for (int j = 0; j < 4; ++j) {
+        if (DT == F32) { const double x = __uint_as_float(r[j]); s = __builtin_fma(x, x, s); }
+        else {
+            const double x = from16(r[j] & 0xFFFFu, DT), y = from16(r[j] >> 16, DT);
+            s = __builtin_fma(x, x, s);
+            s = __builtin_fma(y, y, s);
+        }
+    }
     return s;
 }
-__device__ __forceinline__ double block_sum(double s) {      // 256 threads; the order is fixed
-    __shared__ double part[4];
+// `lanes` lanes, four 16-byte loads of each in flight; lane l of load k takes unit k * lanes + l
+template <int DT>
+__device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, int lanes, int lane) {
+    constexpr int V = DT == F32 ? 4 : 8;
+    const long long at = (long long)tile * (4 * V * lanes), left = e.numel - at;
+    const char* p = (const char*)e.g + at * (16 / V);
+    double s = 0.0;
+    if (left >= 4 * V * lanes) {
+        u32x4 r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = *(const u32x4*)(p + 16 * (size_t)(k * lanes + lane));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s += square_sum16<DT>(r[k]);
+    } else {
+        for (int k = 0; k < 4; ++k) {
+            const long long u = (long long)(k * lanes + lane) * V;
+            if (u + V <= left) s += square_sum16<DT>(*(const u32x4*)(p + u * (16 / V)));
+            else
+                for (long long j = u; j < left && j < u + V; ++j) {
+                    const double x = DT == F32 ? ((const float*)p)[j] : from16(((const uint16_t*)p)[j], DT);
+                    s = __builtin_fma(x, x, s);
+                }
+        }
+    }
+    return s;
+}
+__device__ __forceinline__ double norm_any_tile(const NormTable& t, uint32_t tile, int lanes, int lane) {
+    const int k = __builtin_amdgcn_readfirstlane(find_tensor(t.first, tile));
+    const NormEntry& e = t.e[k];
+    const uint32_t mine = tile - t.first[k];
+    return e.dtype == F32 ? norm_tile<F32>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16>(e, mine, lanes, lane) : norm_tile<F16>(e, mine, lanes, lane);
+}
+template <int WAVES>
+__device__ __forceinline__ double block_sum(double s) {      // complete in thread 0
+    __shared__ double part[WAVES];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) s += __shfl_down(s, off, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    return part[0] + part[1] + part[2] + part[3];
+    if (threadIdx.x == 0) {
+        s = part[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += part[w];
+    }
+    return s;
 }
-// Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split.
+// the norm, and min(1, max_norm / (norm + 1e-6)): NaN when the norm is, as torch.nn.utils.clip_grad_norm_ has it
+__device__ __forceinline__ void norm_results(double sum, double max_norm, float* norm_out, float* clip_out) {
+    const float norm = (float)sqrt(sum);
+    const double c = max_norm / ((double)norm + 1e-6);
+    *norm_out = norm;
+    if (clip_out) *clip_out = max_norm > 0.0 ? (float)(c > 1.0 ? 1.0 : c) : 1.f;
+}
 __global__ __launch_bounds__(256) void grad_norm_kernel(NormTable t, uint32_t tiles, double* partial) {
     double s = 0.0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int k = __builtin_amdgcn_readfirstlane(find_tensor(t.first, tile));
-        const NormEntry& e = t.e[k];
-        const uint32_t mine = tile - t.first[k];
-        const bool full = e.numel - (long long)mine * TILE_ELEMS >= TILE_ELEMS;
-        if (e.dtype == F32) s += full ? norm_tile<F32, true>(e, mine) : norm_tile<F32, false>(e, mine);
-        else if (e.dtype == BF16) s += full ? norm_tile<BF16, true>(e, mine) : norm_tile<BF16, false>(e, mine);
-        else s += full ? norm_tile<F16, true>(e, mine) : norm_tile<F16, false>(e, mine);
-    }
-    s = block_sum(s);
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile(t, tile, 256, threadIdx.x);
+    s = block_sum<4>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
-// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)) (NaN when the norm is, as torch.nn.utils.clip_grad_norm_ has it)
-__global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm, float* out) {
+__global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm, float* norm_out, float* clip_out) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
-    s = block_sum(s);
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(s);
-        const double c = max_norm / ((double)norm + 1e-6);
-        out[0] = norm;
-        out[1] = max_norm > 0.0 ? (float)(c > 1.0 ? 1.0 : c) : 1.f;
-    }
+    for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+    s = block_sum<16>(s);
+    if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
+}
+// few small tensors: one workgroup, a tile per WAVE, no second launch
+__global__ __launch_bounds__(1024) void grad_norm_small_kernel(NormTable t, uint32_t tiles, double max_norm, float* norm_out, float* clip_out) {
+    double s = 0.0;
+    for (uint32_t tile = threadIdx.x >> 6; tile < tiles; tile += 16) s += norm_any_tile(t, tile, 64, threadIdx.x & 63);
+    s = block_sum<16>(s);
+    if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -606,16 +651,25 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
 
 size_t gsicp_grad_norm_scratch_bytes(int n) { return n <= 0 ? 8 : (size_t)((n + NORM_TABLE - 1) / NORM_TABLE) * NORM_GRID * sizeof(double); }
 
-int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* out, void* scratch, void* stream_v) {
+int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
+                    void* stream_v) {
     hipStream_t stream = (hipStream_t)stream_v;
-    if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !out || !scratch) return fail("gsicp_grad_norm: missing arrays");
+    if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !norm_out || !scratch) return fail("gsicp_grad_norm: missing arrays");
+    unsigned long long small = 0;
+    int used_tensors = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || numel[k] >= (1ll << 35)) return fail("gsicp_grad_norm: a tensor has 0 to 2^35 - 1 elements");
-        if (numel[k] > 0 && (!grads[k] || dtype[k] < F32 || dtype[k] > F16)) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
+        if (numel[k] == 0) continue;
+        if (!grads[k] || dtype[k] < F32 || dtype[k] > F16) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
+        ++used_tensors;
+        const int te = norm_tile_elems(dtype[k], 64 * 64);
+        small += (unsigned long long)((numel[k] + te - 1) / te);
     }
+    const bool one = used_tensors <= NORM_TABLE && small <= NORM_SMALL_TILES;
+    const int tile_bytes = one ? 64 * 64 : 256 * 64;
     double* partial = (double*)scratch;
     int used = 0;
-    for (int k = 0; k < n;) {
+    for (int k = 0; k < n || one;) {
         NormTable t = {};
         int m = 0;
         unsigned long long tiles = 0;
@@ -623,16 +677,21 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
             if (numel[k] == 0) continue;
             t.e[m] = {grads[k], numel[k], dtype[k], 0};
             t.first[m++] = (uint32_t)tiles;
-            tiles += tiles_of(numel[k]);
+            const int te = norm_tile_elems(dtype[k], tile_bytes);
+            tiles += (unsigned long long)((numel[k] + te - 1) / te);
             if (tiles > 0xF0000000ull) return fail("gsicp_grad_norm: too many elements in one call");
         }
         for (int i = m; i < 64; ++i) t.first[i] = 0xFFFFFFFFu;
+        if (one) {
+            hipLaunchKernelGGL(grad_norm_small_kernel, dim3(1), dim3(1024), 0, stream, t, (uint32_t)tiles, max_norm, norm_out, clip_out);
+            break;
+        }
         if (m == 0) break;
         const unsigned grid = (unsigned)std::min<unsigned long long>(tiles, NORM_GRID);
         hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
         used += (int)grid;
     }
-    hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)partial, used, max_norm, out);
+    if (!one) hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, stream, (const double*)partial, used, max_norm, norm_out, clip_out);
     if (hipGetLastError() != hipSuccess) { g_last_error = "gsicp_grad_norm: kernel launch failed"; return -1; }
     return 0;
 }

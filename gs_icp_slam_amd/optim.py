@@ -21,7 +21,6 @@ and `FusedAdamW`, the optimiser over them.  `max_norm=` clips by the global norm
 """
 import array
 import ctypes
-import operator
 
 import torch
 
@@ -255,13 +254,22 @@ class FusedAdam(torch.optim.Optimizer):
 
 
 # ------------------------------------------------------------------------------------------------ AdamW over many tensors
-_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _BLOCK = 128                       # elements per base exponent of 8-bit moments
-_numel, _dtype, _device = torch.Tensor.numel, operator.attrgetter("dtype"), operator.attrgetter("device")
+_tensor_lists = None
 
 
-def _addresses(tensors):
-    return array.array("Q", map(torch.Tensor.data_ptr, tensors))
+def _pack(what, names, rules, *lists):
+    """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, n, [addresses of each list], numels, dtype codes, what keeps them alive)."""
+    global _tensor_lists
+    if _tensor_lists is None:
+        try:
+            from . import _tensor_lists as module
+        except ImportError as e:
+            raise ImportError("gs_icp_slam_amd/_tensor_lists not found: build it with `python -m gs_icp_slam_amd.build`") from e
+        _tensor_lists = module
+    device, n, base, keep = _tensor_lists.pack(what, names, rules, *lists)
+    k = len(lists)
+    return device, n, [base + 8 * n * i for i in range(k)], base + 8 * n * k, base + 8 * n * (k + 1), keep
 
 
 def _at(a):
@@ -269,107 +277,77 @@ def _at(a):
     return None if a is None else a.buffer_info()[0]
 
 
-def _check_tensors(what, name, tensors, device, dtypes=None, numels=None):
-    """Lists of contiguous tensors on one HIP device; -> their dtypes.  Works on whole lists: a step over hundreds of small tensors is bound by the host."""
-    for d in set(map(_device, tensors)):
-        if d != device or not device.type == "cuda":
-            raise RuntimeError(f"{what} (gfx950): {name} must live on one HIP device (found {d}); there is no CPU path")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
-        raise RuntimeError(f"{what}: {name} must be contiguous")
-    found = list(map(_dtype, tensors))
-    if dtypes is not None and found != dtypes:
-        raise RuntimeError(f"{what}: {name} have the wrong dtype ({', '.join(sorted({str(t) for t in set(found) - set(dtypes)} or {'mixed up'}))})")
-    if numels is not None and list(map(_numel, tensors)) != numels:
-        raise RuntimeError(f"{what}: {name} have the wrong number of elements")
-    return found
-
-
-def _codes(what, name, dtypes):
-    try:
-        return array.array("i", map(_DTYPE_CODE.__getitem__, dtypes))
-    except KeyError as e:
-        raise RuntimeError(f"{what}: {name} must be float32, bfloat16 or float16 (found {e.args[0]})") from None
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _doubles(what, name, value, n):
     if isinstance(value, (int, float)):
-        return array.array("d", [value]) * n
+        return array.array("d", (value,)) * n
     a = array.array("d", value)
     if len(a) != n:
         raise RuntimeError(f"{what}: {name} is a number or one per tensor ({len(a)} for {n} tensors)")
     return a
 
 
-def _norm_launch(what, addresses, numels, codes, device, max_norm):
-    """-> f32[2] on the device: the norm and the clip factor (1 without a max_norm)."""
+def _call(fn, name, device, *args):
+    """fn(*args, current stream of `device`) with that device current."""
+    if torch.cuda.current_device() == device:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc < 0:
+        _lib.check(rc, name)
+
+
+def _norm(what, device, n, addresses, numels, codes, max_norm):
+    """-> (norm: 0-dim f32 on the device, scratch whose first word is the clip factor)."""
     if max_norm is None:
         max_norm = 0.0
     elif not max_norm > 0.0:
         raise RuntimeError(f"{what}: max_norm must be positive")
     lib = _lib.load()
-    n = len(addresses)
-    out = torch.empty(2, dtype=torch.float32, device=device)
-    scratch = torch.empty(int(lib.gsicp_grad_norm_scratch_bytes(n)), dtype=torch.uint8, device=device)
-    with torch.cuda.device(device):
-        _lib.check(lib.gsicp_grad_norm(n, _at(addresses), _at(numels), _at(codes), float(max_norm), out.data_ptr(), scratch.data_ptr(), _stream(device)), "gsicp_grad_norm")
-    return out
+    dev = torch.device("cuda", device)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    size = int(lib.gsicp_grad_norm_scratch_bytes(n))
+    scratch = torch.empty(size + 8, dtype=torch.uint8, device=dev)
+    at = scratch.data_ptr()
+    _call(lib.gsicp_grad_norm, "gsicp_grad_norm", device, n, addresses, numels, codes, float(max_norm), norm.data_ptr(), at, at + 8)
+    return norm, scratch
 
 
 def grad_norm(tensors):
     """2-norm over all elements of `tensors` (f32, bf16 or f16, mixed, any sizes, contiguous, one device) as a 0-dim f32 tensor on their device; nothing synchronises.
     Squares and sums are taken in double and in a fixed order: the same tensors give the same bits."""
-    tensors = list(tensors)
-    if not tensors:
-        raise RuntimeError("grad_norm: no tensors")
-    device = tensors[0].device
-    codes = _codes("grad_norm", "tensors", _check_tensors("grad_norm", "tensors", tensors, device))
-    return _norm_launch("grad_norm", _addresses(tensors), array.array("q", map(_numel, tensors)), codes, device, None)[0]
+    device, n, (g,), numels, codes, keep = _pack("grad_norm", ("tensors",), "p", list(tensors))
+    return _norm("grad_norm", device, n, g, numels, codes, None)[0]
 
 
-def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, betas, eps, step, max_norm=None, norm=None, seed=0, place=None, device_form=None):
-    """Checks, lays out and launches a step of either form; -> the norm and clip factor (f32[2] on the device) or None.  norm: one taken before (max_norm is then not
-    looked at); device_form(n): the gsicp_adamw_device of a captured step, and what it points to."""
-    n = len(params)
-    device = params[0].device
-    if not len(grads) == len(first) == len(second) == n or (masters is not None and len(masters) != n):
-        raise RuntimeError(f"{what}: {n} parameters, {len(grads)} gradients, {len(first)} and {len(second)} moments" + ("" if masters is None else f", {len(masters)} masters"))
-    dtypes = _check_tensors(what, "parameters", params, device)
-    numels = list(map(_numel, params))
-    _check_tensors(what, "gradients", grads, device, dtypes, numels)
-    codes = _codes(what, "parameters", dtypes)
-    if bits == 32:
-        f32 = [torch.float32] * n
-        _check_tensors(what, "exp_avgs", first, device, f32, numels)
-        _check_tensors(what, "exp_avg_sqs", second, device, f32, numels)
+_NAMES_32, _NAMES_8 = ("parameters", "gradients", "exp_avgs", "exp_avg_sqs"), ("parameters", "gradients", "moments", "block_exps")
+_NAMES_32_MASTERS, _NAMES_8_MASTERS = _NAMES_32 + ("masters",), _NAMES_8 + ("masters",)
+
+
+def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, betas, eps, step, max_norm=None, clip=None, seed=0, place=None, device_form=None):
+    """Checks, lays out and launches a step of either form; -> the norm or None.  clip: device address of a factor taken before (max_norm is then not looked at);
+    device_form(): the gsicp_adamw_device of a captured step and what it points to."""
+    if masters is None:
+        device, n, (p, g, s0, s1), numels, codes, keep = _pack(what, _NAMES_32 if bits == 32 else _NAMES_8, "pgff" if bits == 32 else "pghb", params, grads, first, second)
+        mast = None
     else:
-        i16 = [torch.int16] * n
-        _check_tensors(what, "moments", first, device, i16, numels)
-        _check_tensors(what, "block_exps", second, device, i16, [(k + _BLOCK - 1) // _BLOCK for k in numels])
-    master_at = None
-    if masters is not None:
-        given = [m for m in masters if m is not None]
-        _check_tensors(what, "masters", given, device, [torch.float32] * len(given), [k for k, m in zip(numels, masters) if m is not None])
-        master_at = array.array("Q", [0 if m is None else m.data_ptr() for m in masters])
-    param_at, grad_at, first_at, second_at, numel_at = _addresses(params), _addresses(grads), _addresses(first), _addresses(second), array.array("q", numels)
-    lr = None if device_form else _doubles(what, "lr", lr, n)
+        device, n, (p, g, s0, s1, mast), numels, codes, keep = _pack(what, _NAMES_32_MASTERS if bits == 32 else _NAMES_8_MASTERS, "pgffm" if bits == 32 else "pghbm",
+                                                                     params, grads, first, second, masters)
     weight_decay = _doubles(what, "weight_decay", weight_decay, n)
-    if norm is None and max_norm is not None:
-        norm = _norm_launch(what, grad_at, numel_at, codes, device, max_norm)
-    clip = None if norm is None else norm.data_ptr() + 4
-    dev, keep = (None, None) if device_form is None else device_form(n)
-    args = [n, _at(param_at), _at(grad_at), _at(master_at), _at(first_at), _at(second_at), _at(numel_at), _at(codes), _at(lr), _at(weight_decay), betas[0], betas[1], eps,
-            int(step)]
+    if device_form is None:
+        lr, dev, dev_keep = _doubles(what, "lr", lr, n), None, None
+    else:
+        lr, (dev, dev_keep) = None, device_form()
+    norm = scratch = None
+    if clip is None and max_norm is not None:
+        norm, scratch = _norm(what, device, n, g, numels, codes, max_norm)
+        clip = scratch.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(device):
-        if bits == 32:
-            _lib.check(lib.gsicp_adamw_step(*args, clip, dev, _stream(device)), "gsicp_adamw_step")
-        else:
-            _lib.check(lib.gsicp_adamw_step_8bit(*args, int(seed) & 0xFFFFFFFF, _at(place), clip, dev, _stream(device)), "gsicp_adamw_step_8bit")
-    del keep
+    if bits == 32:
+        _call(lib.gsicp_adamw_step, "gsicp_adamw_step", device, n, p, g, mast, s0, s1, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step), clip, dev)
+    else:
+        _call(lib.gsicp_adamw_step_8bit, "gsicp_adamw_step_8bit", device, n, p, g, mast, s0, s1, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step),
+              int(seed) & 0xFFFFFFFF, _at(place), clip, dev)
     return norm
 
 
@@ -383,8 +361,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr, step, betas=(0.9, 0.
     params = list(params)
     if not params:
         return None
-    norm = _adamw("adamw_step", 32, params, list(grads), masters, list(exp_avgs), list(exp_avg_sqs), lr, weight_decay, betas, eps, step, max_norm)
-    return None if norm is None else norm[0]
+    return _adamw("adamw_step", 32, params, grads, masters, exp_avgs, exp_avg_sqs, lr, weight_decay, betas, eps, step, max_norm)
 
 
 def adamw_step_8bit(params, grads, moments, block_exps, *, lr, step, seed=0, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, max_norm=None):
@@ -393,8 +370,7 @@ def adamw_step_8bit(params, grads, moments, block_exps, *, lr, step, seed=0, bet
     params = list(params)
     if not params:
         return None
-    norm = _adamw("adamw_step_8bit", 8, params, list(grads), masters, list(moments), list(block_exps), lr, weight_decay, betas, eps, step, max_norm, seed=seed)
-    return None if norm is None else norm[0]
+    return _adamw("adamw_step_8bit", 8, params, grads, masters, moments, block_exps, lr, weight_decay, betas, eps, step, max_norm, seed=seed)
 
 
 def new_moments_8bit(param):
@@ -408,18 +384,13 @@ def decode_moments(moments, block_exps, dtype=torch.float32):
     moments, block_exps = list(moments), list(block_exps)
     if not moments:
         return [], []
-    what = "decode_moments"
     if dtype not in (torch.float32, torch.bfloat16):
-        raise RuntimeError(f"{what}: dtype is float32 or bfloat16")
-    device, n = moments[0].device, len(moments)
-    _check_tensors(what, "moments", moments, device, [torch.int16] * n)
-    numels = list(map(_numel, moments))
-    _check_tensors(what, "block_exps", block_exps, device, [torch.int16] * n, [(k + _BLOCK - 1) // _BLOCK for k in numels])
-    exp_avgs = [torch.empty(t.shape, dtype=dtype, device=device) for t in moments]
-    exp_avg_sqs = [torch.empty(t.shape, dtype=dtype, device=device) for t in moments]
-    c, b, m, v, k = _addresses(moments), _addresses(block_exps), _addresses(exp_avgs), _addresses(exp_avg_sqs), array.array("q", numels)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().gsicp_adamw_decode(n, _at(c), _at(b), _at(m), _at(v), _at(k), _DTYPE_CODE[dtype], _stream(device)), "gsicp_adamw_decode")
+        raise RuntimeError("decode_moments: dtype is float32 or bfloat16")
+    device, n, (c, e), numels, _, keep = _pack("decode_moments", ("moments", "block_exps"), "cb", moments, block_exps)
+    exp_avgs = [torch.empty(t.shape, dtype=dtype, device=t.device) for t in moments]
+    exp_avg_sqs = [torch.empty(t.shape, dtype=dtype, device=t.device) for t in moments]
+    m, v = (array.array("Q", [t.data_ptr() for t in ts]) for ts in (exp_avgs, exp_avg_sqs))
+    _call(_lib.load().gsicp_adamw_decode, "gsicp_adamw_decode", device, n, c, e, _at(m), _at(v), numels, int(dtype == torch.bfloat16))
     return exp_avgs, exp_avg_sqs
 
 
@@ -529,17 +500,15 @@ class FusedAdamW(FusedAdam):
                     st["step"] = fresh.setdefault((int(st["step"]), p.device), torch.full((), int(st["step"]), dtype=torch.int32, device=p.device))
                 key = (float(b1), float(b2), float(group["eps"]), st["step"].data_ptr() if self.capturable else int(st["step"]), p.device)
                 buckets.setdefault(key, []).append((p, p.grad.contiguous(), st, gi, pi, place))
-        norm = None
+        clip = scratch = None
         if self.max_grad_norm is not None and buckets:
             if self._grad_rows is not None:
                 raise RuntimeError("FusedAdamW: max_grad_norm reads every gradient row, set_grad_row_mask says some were not written")
             if len({key[4] for key in buckets}) > 1:
                 raise RuntimeError("FusedAdamW(max_grad_norm): the parameters live on several devices")
-            grads = [t[1] for items in buckets.values() for t in items]
-            device = grads[0].device
-            codes = _codes("FusedAdamW", "gradients", _check_tensors("FusedAdamW", "gradients", grads, device))
-            norm = _norm_launch("FusedAdamW", _addresses(grads), array.array("q", map(_numel, grads)), codes, device, self.max_grad_norm)
-            self.last_grad_norm = norm[0]
+            device, n, (g,), numels, codes, keep = _pack("FusedAdamW", ("gradients",), "p", [t[1] for items in buckets.values() for t in items])
+            self.last_grad_norm, scratch = _norm("FusedAdamW", device, n, g, numels, codes, self.max_grad_norm)
+            clip = scratch.data_ptr()
         last_of = {key[3:]: key for key in buckets}         # a device counter is advanced by the last launch that reads it
         first, second = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
         for key, items in buckets.items():
@@ -548,10 +517,10 @@ class FusedAdamW(FusedAdam):
             device_form = None
             if self.capturable:
                 bump = 2 if step_already_bumped else int(last_of[key[3:]] == key)
-                device_form = lambda n, items=items, key=key, bump=bump: self._device_form(items, key, bump)   # noqa: E731
+                device_form = lambda items=items, key=key, bump=bump: self._device_form(items, key, bump)   # noqa: E731
             _adamw("FusedAdamW", self.state_bits, [t[0] for t in items], [t[1] for t in items], masters if any(m is not None for m in masters) else None,
                    [t[2][first] for t in items], [t[2][second] for t in items], [float(g["lr"]) for g in groups], [float(g["weight_decay"]) for g in groups], key[:2], key[2],
-                   1 if self.capturable else key[3] + 1, norm=norm, seed=self.seed, place=array.array("i", [t[5] for t in items]), device_form=device_form)
+                   1 if self.capturable else key[3] + 1, clip=clip, seed=self.seed, place=array.array("i", [t[5] for t in items]), device_form=device_form)
             if not self.capturable:
                 for t in items:
                     t[2]["step"] = key[3] + 1
@@ -559,7 +528,7 @@ class FusedAdamW(FusedAdam):
 
     def _device_form(self, items, key, bump):
         """The gsicp_adamw_device of one captured launch sequence, and the host arrays it points to."""
-        device, n = key[4], len(items)
+        device = key[4]
         ids = tuple((t[3], t[4]) for t in items)
         lrs = [float(self.param_groups[gi]["lr"]) for gi, _ in ids]
         entry = self._lr_dev.get((ids,) + key[:3])

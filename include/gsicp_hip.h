@@ -413,7 +413,7 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
  * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
  * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 is
  * allowed, < 2^35), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap (checked; -2).
- * clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's out + 1), or NULL.  step: the 1-based count after the increment.
+ * clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's clip_out), or NULL.  step: the 1-based count after the increment.
  * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (live_rows and the row masks: f32
  * parameters of < 2^32 elements). */
 typedef struct {
@@ -444,10 +444,12 @@ int gsicp_adamw_step_8bit(int n, void* const* params, const void* const* grads, 
 /* Values of 8-bit moments, as f32 (dtype 0) or bf16 (1; exact). */
 int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* const* block_exps, void* const* exp_avg, void* const* exp_avg_sq, const long long* numel,
                        int dtype, void* stream);
-/* out[0] = 2-norm over all elements of n tensors (dtype[k] as above; squares and sums in double, fixed order), out[1] = min(1, max_norm / (norm + 1e-6)) — the factor of
- * torch.nn.utils.clip_grad_norm_ —, or 1 when max_norm <= 0.  out: DEVICE float[2]; scratch: DEVICE, gsicp_grad_norm_scratch_bytes(n), needs no initialisation. */
+/* *norm_out = 2-norm over all elements of n tensors (dtype[k] as above; squares and sums in double, fixed order), *clip_out (may be NULL) = min(1, max_norm /
+ * (norm + 1e-6)) — the factor of torch.nn.utils.clip_grad_norm_ —, or 1 when max_norm <= 0.  norm_out, clip_out: DEVICE; scratch: DEVICE, 8-byte aligned,
+ * gsicp_grad_norm_scratch_bytes(n) bytes, needs no initialisation and holds nothing afterwards. */
 size_t gsicp_grad_norm_scratch_bytes(int n);
-int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* out, void* scratch, void* stream);
+int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
+                    void* stream);
 
 /* Map pruning without reallocation: GaussianModel.prune_points / _prune_optimizer
  * [REF scene/gaussian_model.py:409-447] apply one boolean mask to every parameter, both Adam moments and the per-Gaussian

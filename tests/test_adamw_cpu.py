@@ -122,10 +122,10 @@ def test_c_abi_refuses_before_it_launches():
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(0), k(5), 0, None) == -2
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(64), k(5), 2, None) == -2
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(64), k(-5), 0, None) == -2
-    assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(0), 0.0, None, 64, None) == -2
-    assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(5), 0.0, 64, 64, None) == -2
-    assert lib.gsicp_grad_norm(1, one(0), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, None) == -2
-    assert lib.gsicp_grad_norm(1, one(64), k(1 << 35), (ctypes.c_int * 1)(0), 0.0, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(0), 0.0, None, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(5), 0.0, 64, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(0), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(64), k(1 << 35), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm_scratch_bytes(0) > 0 and lib.gsicp_grad_norm_scratch_bytes(65) > lib.gsicp_grad_norm_scratch_bytes(64)
 
 

@@ -21,12 +21,11 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <string>
 #include <utility>
 #include <vector>
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include "../../include/gsicp_hip.h"
@@ -39,17 +38,18 @@ namespace {
 
 constexpr int TABLE = 40;             // tensors per launch: the table travels in the kernel arguments (< 4 KB), nothing is copied or kept
 constexpr int NORM_TABLE = 64;
-constexpr int TILE_ELEMS = 2048;      // elements per workgroup and pass: 256 lanes x 8
-constexpr int STEP_GRID = 2048;       // workgroups of a large launch (8 per CU)
+constexpr uint32_t LAST = 0x7FFFFFFF; // a tile number that no launch reaches
+constexpr int TILE_ELEMS = 256;       // elements of a workgroup of the step and of the decoding: ONE wave, four consecutive elements a lane, no loop
 constexpr int NORM_GRID = 2048;       // partial sums of one norm launch
 constexpr int NORM_SMALL_TILES = 128; // 4 KB tiles that one workgroup of 16 waves takes by itself
-constexpr int QBLOCK = 128;           // elements per base exponent: 16 lanes x 8
+constexpr int QBLOCK = 128;           // elements per base exponent: 32 lanes x 4
 
 enum Dtype { F32 = 0, BF16 = 1, F16 = 2 };
 
 // vector types without an alignment demand beyond the element's: views of a flat buffer begin anywhere
 typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(2)));
 
 struct StepEntry {
     void* p;
@@ -58,26 +58,27 @@ struct StepEntry {
     void* s1;              // exp_avg_sq, or the base exponents
     float* master;
     long long numel;
-    double lr, wd;
+    float step_size, decay;     // lr / (1 - b1^t) and 1 - lr wd   (host form)
+    double wd;                  // the device form takes lr from memory
+    uint32_t first;             // its first tile
     int row_width;         // elements per map row (live rows, masks); 0: whole tensor
     uint16_t kind;         // Dtype | 4 with a master
     uint16_t frozen;       // rows with a non-zero freeze word are left alone
     int src, place;        // index in the caller's arrays (device learning rates), place in the list (random bits)
 };
 struct StepTable {
-    uint32_t first[64];    // first tile of each tensor; ~0 behind the last: a wave finds the tensor of a tile by one ballot
+    uint32_t first[64];    // first tile of each tensor; LAST behind them
     StepEntry e[TABLE];
 };
 struct StepHyper {
     float b1, omb1, b2, omb2, eps;
     float inv_bc2_sqrt;    // 1 / sqrt(1 - b2^t)            (host step count)
-    double inv_bc1;        // 1 / (1 - b1^t)
-    double db1, db2;       // for the same on the device     (device step count)
+    double log2_b1, log2_b2;   // for the same on the device     (device step count)
     const float* clip;     // device: the factor of every gradient (NULL: 1)
     const double* lr_dev;
     const int* step_dev;
     int step;              // host: the step count; device: what to add to *step_dev
-    uint32_t seed, tiles;
+    uint32_t seed;
     const uint32_t* guard_count;
     uint32_t guard_limit;
     const int *live_rows, *row_freeze, *grad_rows;
@@ -94,115 +95,142 @@ __device__ __forceinline__ uint32_t lane_word(int e) {
     return w[e];
 }
 
-// the tensor a tile belongs to: lane l compares the tile with tensor l's first one
-__device__ __forceinline__ int find_tensor(const uint32_t* first, uint32_t tile) {
-    return __popcll(__ballot(first[threadIdx.x & 63] <= tile)) - 1;
+// The tensor a tile belongs to: the number of first tiles at or before it, less one.  `first` lies in the kernel arguments and `tile` is the same for the wave, so all of this is
+// scalar: sixteen entries a load, and the scalar cache answers while the vector path is full of the other waves' streams.
+// Tile numbers are below 2^31: the sign of first - tile - 1 is the comparison (a boolean sum would go through vector registers).
+__device__ __forceinline__ uint32_t find_tensor(const uint32_t* first, uint32_t tile) {
+    uint32_t k = 0;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) k += (first[i] + ~tile) >> 31;
+    if (tile >= first[16]) {
+        k = 16 + 16 * (((first[32] + ~tile) >> 31) + ((first[48] + ~tile) >> 31));
+        const uint32_t* f = first + k;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) k += (f[i] + ~tile) >> 31;
+    }
+    return k;
 }
+// Demands a wave-uniform value here, in scalar registers: without it the compiler moves each load of a table entry to its first use, and the wave waits for them one by one.
+template <class T> __device__ __forceinline__ void at_hand(T x) { asm volatile("" : : "s"(x)); }
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float from16(uint32_t h, int dtype) {
-    return dtype == BF16 ? __uint_as_float(h << 16) : __half2float(__ushort_as_half((unsigned short)h));
+    return dtype == BF16 ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
-__device__ __forceinline__ uint32_t to16(float x, int dtype) {        // round to nearest, ties to even
-    if (dtype == F16) return __half_as_ushort(__float2half_rn(x));
-    const uint32_t b = __float_as_uint(x);
-    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (b >> 16) | 0x40u;    // NaN stays NaN
-    return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+// two values, the first in the low half; round to nearest, ties to even
+__device__ __forceinline__ uint32_t to16x2(float x, float y, int dtype) {
+    const f32x2 f = {x, y};
+    if (dtype == F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
 }
 
-// eight consecutive elements; FULL: all of them exist, else only the first nv
-template <int DT, bool FULL>
-__device__ __forceinline__ void load8(const void* base, long long at, int nv, float out[8]) {
+// one overload per vector type: a deduced type would lose the element's alignment
+#define GSICP_ACCESS(V)                                                                                                          \
+    template <bool NT> __device__ __forceinline__ V get(const V* p) { return NT ? __builtin_nontemporal_load(p) : *p; }           \
+    template <bool NT> __device__ __forceinline__ void put(V* p, V v) { if (NT) __builtin_nontemporal_store(v, p); else *p = v; }
+GSICP_ACCESS(f32x4)
+GSICP_ACCESS(u32x4)
+GSICP_ACCESS(u32x2)
+#undef GSICP_ACCESS
+
+// four consecutive elements; FULL: all of them exist, else only the first nv
+template <int DT, bool FULL, bool NT>
+__device__ __forceinline__ void load4(const void* base, long long at, int nv, float out[4]) {
     if (DT == F32) {
         const float* p = (const float*)base + at;
         if (FULL) {
-            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+            const f32x4 a = get<NT>((const f32x4*)p);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { out[j] = a[j]; out[j + 4] = b[j]; }
+            for (int j = 0; j < 4; ++j) out[j] = a[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = j < nv ? p[j] : 0.f;
+            for (int j = 0; j < 4; ++j) out[j] = j < nv ? p[j] : 0.f;
         }
     } else {
         const uint16_t* p = (const uint16_t*)base + at;
         if (FULL) {
-            const u32x4 a = *(const u32x4*)p;
+            const u32x2 a = get<NT>((const u32x2*)p);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = from16((a[j >> 1] >> (16 * (j & 1))) & 0xFFFFu, DT);
+            for (int j = 0; j < 4; ++j) out[j] = from16((a[j >> 1] >> (16 * (j & 1))) & 0xFFFFu, DT);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = j < nv ? from16(p[j], DT) : 0.f;
+            for (int j = 0; j < 4; ++j) out[j] = j < nv ? from16(p[j], DT) : 0.f;
         }
     }
 }
-template <int DT, bool FULL>
-__device__ __forceinline__ void store8(void* base, long long at, int nv, const float x[8]) {
+template <int DT, bool FULL, bool NT>
+__device__ __forceinline__ void store4(void* base, long long at, int nv, const float x[4]) {
     if (DT == F32) {
         float* p = (float*)base + at;
         if (FULL) {
-            f32x4 a, b;
+            f32x4 a;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { a[j] = x[j]; b[j] = x[j + 4]; }
-            *(f32x4*)p = a;
-            *(f32x4*)(p + 4) = b;
+            for (int j = 0; j < 4; ++j) a[j] = x[j];
+            put<NT>((f32x4*)p, a);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (j < nv) p[j] = x[j];
+            for (int j = 0; j < 4; ++j) if (j < nv) p[j] = x[j];
         }
     } else {
         uint16_t* p = (uint16_t*)base + at;
         if (FULL) {
-            u32x4 a;
+            u32x2 a;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = to16(x[2 * j], DT) | (to16(x[2 * j + 1], DT) << 16);
-            *(u32x4*)p = a;
+            for (int j = 0; j < 2; ++j) a[j] = to16x2(x[2 * j], x[2 * j + 1], DT);
+            put<NT>((u32x2*)p, a);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (j < nv) p[j] = (uint16_t)to16(x[j], DT);
+            for (int j = 0; j < 4; ++j) if (j < nv) p[j] = (uint16_t)to16x2(x[j], 0.f, DT);
         }
     }
 }
-template <bool FULL>
-__device__ __forceinline__ void load_codes(const void* base, long long at, int nv, uint32_t c[4]) {
+template <bool FULL, bool NT>
+__device__ __forceinline__ void load_codes(const void* base, long long at, int nv, uint32_t c[2]) {
     const uint16_t* p = (const uint16_t*)base + at;
     if (FULL) {
-        const u32x4 a = *(const u32x4*)p;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = a[j];
+        const u32x2 a = get<NT>((const u32x2*)p);
+        c[0] = a[0]; c[1] = a[1];
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = (2 * j < nv ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < nv ? (uint32_t)p[2 * j + 1] << 16 : 0u);
+        for (int j = 0; j < 2; ++j) c[j] = (2 * j < nv ? (uint32_t)p[2 * j] : 0u) | (2 * j + 1 < nv ? (uint32_t)p[2 * j + 1] << 16 : 0u);
     }
 }
-template <bool FULL>
-__device__ __forceinline__ void store_codes(void* base, long long at, int nv, const uint32_t c[4]) {
+template <bool FULL, bool NT>
+__device__ __forceinline__ void store_codes(void* base, long long at, int nv, const uint32_t c[2]) {
     uint16_t* p = (uint16_t*)base + at;
     if (FULL) {
-        u32x4 a;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = c[j];
-        *(u32x4*)p = a;
+        u32x2 a;
+        a[0] = c[0]; a[1] = c[1];
+        put<NT>((u32x2*)p, a);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < nv) p[j] = (uint16_t)(c[j >> 1] >> (16 * (j & 1)));
+        for (int j = 0; j < 4; ++j) if (j < nv) p[j] = (uint16_t)(c[j >> 1] >> (16 * (j & 1)));
     }
 }
 
 __device__ __forceinline__ float decode_m(uint32_t c16, uint32_t bm23) {
     const uint32_t mag = c16 & 0x7Fu;
-    const uint32_t bits = ((mag << 20) + bm23) | ((c16 & 0x80u) << 24);
-    return mag == 0u ? 0.f : __uint_as_float(mag == 127u ? 0x7FC00000u : bits);
+    uint32_t bits = (c16 << 24 & 0x80000000u) | ((mag << 20) + bm23);
+    bits = mag == 127u ? 0x7FC00000u : bits;
+    return __uint_as_float(mag == 0u ? 0u : bits);
 }
 __device__ __forceinline__ float decode_v(uint32_t c16, uint32_t bv23) {
-    const uint32_t c = (c16 >> 8) & 0xFFu;
-    return c == 0u ? 0.f : __uint_as_float(c == 255u ? 0x7F800000u : (c << 20) + bv23);
+    const uint32_t c = c16 >> 8 & 0xFFu;
+    uint32_t bits = (c << 20) + bv23;
+    bits = c == 255u ? 0x7F800000u : bits;
+    return __uint_as_float(c == 0u ? 0u : bits);
 }
-// largest value of the 16 lanes of a row, in every one of them: four rotations
-__device__ __forceinline__ uint32_t row16_max(uint32_t x) {
+// largest value of each half of the wave, in every lane of it: four rotations within rows of 16, one exchange of neighbouring rows
+__device__ __forceinline__ uint32_t half_max(uint32_t x) {
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xF, 0xF, true));   // row_ror:8
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xF, 0xF, true));   // row_ror:4
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xF, 0xF, true));   // row_ror:2
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xF, 0xF, true));   // row_ror:1
-    return x;
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
 }
 __device__ __forceinline__ uint32_t base_exponent(uint32_t top, int below) {
     const int b = (int)(top >> 23) - below;
@@ -212,28 +240,71 @@ __device__ __forceinline__ uint32_t base_exponent(uint32_t top, int below) {
 // what one step needs to know of a tensor, after the hyper-parameters are folded
 struct Fold { float b1, omb1, b2, omb2, eps, ibc2, decay, step_size, clip; };
 
-__device__ __forceinline__ void adamw(float& p, float& m, float& v, float g, const Fold& f) {
-    m = m * f.b1 + g * f.omb1;
-    v = v * f.b2 + g * f.omb2 * g;
-    p = p * f.decay;
-    p = p - f.step_size * (m / (sqrtf(v) * f.ibc2 + f.eps));
+// Four elements.  The moments round operation by operation; the parameter takes the hardware's root and reciprocal (measured over all exponents: off by less than 1.6 * 2^-24 of the
+// result each, where the correctly rounded sequences cost 25 instructions an element) and fused sums.  The hardware's root takes a subnormal for zero: a wave that holds a
+// subnormal second moment goes the long way.
+__device__ __forceinline__ void adamw4(float p[4], float m[4], float v[4], const float g[4], const Fold& f) {
+    bool subnormal = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        m[j] = m[j] * f.b1 + g[j] * f.omb1;
+        v[j] = v[j] * f.b2 + g[j] * f.omb2 * g[j];
+        subnormal |= __builtin_amdgcn_classf(v[j], 0x80);
+    }
+    float root[4];
+    if (__ballot(subnormal) == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) root[j] = __builtin_amdgcn_sqrtf(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) root[j] = sqrtf(v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        p[j] = __builtin_fmaf(-f.step_size, m[j] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[j], f.ibc2, f.eps)), p[j] * f.decay);
 }
 
-template <bool Q8, int DT, bool MASTER, bool FULL, bool MASKED>
+// New moments -> codes.  SPECIAL: some value of the wave is not finite.  top_m, top_v: bits of the largest value of the lane's block.
+template <bool SPECIAL>
+__device__ __forceinline__ void encode4(const float m[4], const float v[4], uint32_t bm, uint32_t bv, uint32_t word, uint32_t o[2]) {
+    const float low = __uint_as_float((bm << 23) + (1u << 20)), low16 = low * 0x1p-16f, low17 = low16 * 0.5f;
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t r = word * ((threadIdx.x & 1) ? lane_word(j + 4) : lane_word(j));
+        const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = SPECIAL ? __float_as_uint(v[j]) & 0x7FFFFFFFu : __float_as_uint(v[j]);
+        const float a = __uint_as_float(mb);
+        uint32_t mc = ((mb + ((r << 4 & 0xFFFF0u) | 8u)) >> 20) - (bm << 3);
+        // fma: low16 * (u + 1/2), rounded once
+        mc = a < low ? (a > __builtin_fmaf(low16, (float)(r & 0xFFFFu), low17) ? 1u : 0u) : mc;
+        mc = (__float_as_uint(m[j]) >> 24 & 0x80u) | mc;
+        const int vs = (int)((vb + ((r >> 12 & 0xFFFF0u) | 8u)) >> 20) - (int)(bv << 3);
+        uint32_t vc = vb == 0u ? 0u : (uint32_t)max(vs, 1);
+        if (SPECIAL) {
+            if (mb >= 0x7F800000u) mc = 127u;
+            if (vb >= 0x7F800000u) vc = 255u;
+        }
+        h[j] = vc << 8 | mc;
+    }
+    o[0] = h[1] << 16 | h[0];
+    o[1] = h[3] << 16 | h[2];
+}
+
+template <bool Q8, int DT, bool MASTER, bool FULL, bool MASKED, bool NT>
 __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, const int* row_freeze, const int* grad_rows, uint32_t key, uint32_t tile, long long numel) {
-    const long long at = (long long)tile * TILE_ELEMS + 8 * threadIdx.x;
-    const int nv = FULL ? 8 : (int)max(0ll, min(8ll, numel - at));
-    float p[8], g[8], m[8], v[8];
-    uint32_t c[4], exps = 0;
-    if (MASTER) load8<F32, FULL>(e.master, at, nv, p); else load8<DT, FULL>(e.p, at, nv, p);
-    load8<DT, FULL>(e.g, at, nv, g);
-    const long long block = (long long)tile * (TILE_ELEMS / QBLOCK) + (threadIdx.x >> 4);
+    const long long at = (long long)tile * TILE_ELEMS + 4 * threadIdx.x;
+    const int nv = FULL ? 4 : (int)max(0ll, min(4ll, numel - at));
+    float p[4], g[4], m[4], v[4];
+    uint32_t c[2], exps = 0;
+    if (MASTER) load4<F32, FULL, NT>(e.master, at, nv, p); else load4<DT, FULL, NT>(e.p, at, nv, p);
+    load4<DT, FULL, NT>(e.g, at, nv, g);
+    const long long block = (long long)tile * (TILE_ELEMS / QBLOCK) + (threadIdx.x >> 5);
     if (Q8) {
-        load_codes<FULL>(e.s0, at, nv, c);
+        load_codes<FULL, NT>(e.s0, at, nv, c);
         if (FULL || nv > 0) exps = ((const uint16_t*)e.s1)[block];
     } else {
-        load8<F32, FULL>(e.s0, at, nv, m);
-        load8<F32, FULL>(e.s1, at, nv, v);
+        load4<F32, FULL, NT>(e.s0, at, nv, m);
+        load4<F32, FULL, NT>(e.s1, at, nv, v);
     }
     uint32_t keep = 0;                          // elements of frozen rows
     if (MASKED) {
@@ -241,7 +312,7 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
         if (w && nv > 0) {
             uint32_t row = (uint32_t)at / w, col = (uint32_t)at - row * w;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 if (FULL || j < nv) {
                     if (grad_rows && grad_rows[row] <= 0) g[j] = 0.f;     // whatever the gradient's memory holds there
                     if (e.frozen && row_freeze[row] != 0) keep |= 1u << j;
@@ -251,107 +322,107 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
         }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] *= f.clip;
+    for (int j = 0; j < 4; ++j) g[j] *= f.clip;
     if (Q8) {
         const uint32_t bm23 = (exps & 0xFFu) << 23, bv23 = (exps >> 8) << 23;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
             const uint32_t c16 = c[j >> 1] >> (16 * (j & 1));
             m[j] = decode_m(c16, bm23);
             v[j] = decode_v(c16, bv23);
         }
     }
-    float p0[8], m0[8], v0[8];
+    float p0[4], m0[4], v0[4];
     if (MASKED && !Q8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { p0[j] = p[j]; m0[j] = m[j]; v0[j] = v[j]; }
+        for (int j = 0; j < 4; ++j) { p0[j] = p[j]; m0[j] = m[j]; v0[j] = v[j]; }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) adamw(p[j], m[j], v[j], g[j], f);
+    adamw4(p, m, v, g, f);
     if (MASKED && !Q8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (keep >> j & 1u) { p[j] = p0[j]; m[j] = m0[j]; v[j] = v0[j]; }
+        for (int j = 0; j < 4; ++j) if (keep >> j & 1u) { p[j] = p0[j]; m[j] = m0[j]; v[j] = v0[j]; }
     }
-    if (MASTER) store8<F32, FULL>(e.master, at, nv, p);
-    store8<DT, FULL>(e.p, at, nv, p);
+    if (MASTER) store4<F32, FULL, NT>(e.master, at, nv, p);
+    store4<DT, FULL, NT>(e.p, at, nv, p);
     if (!Q8) {
-        store8<F32, FULL>(e.s0, at, nv, m);
-        store8<F32, FULL>(e.s1, at, nv, v);
+        store4<F32, FULL, NT>(e.s0, at, nv, m);
+        store4<F32, FULL, NT>(e.s1, at, nv, v);
         return;
     }
     uint32_t tm = 0, tv = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+    for (int j = 0; j < 4; ++j)
         if (FULL || j < nv) {
-            tm = max(tm, mb < 0x7F800000u ? mb : 0u);
-            tv = max(tv, vb < 0x7F800000u ? vb : 0u);
+            tm = max(tm, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+            tv = max(tv, __float_as_uint(v[j]));
         }
-    }
-    const uint32_t bm = base_exponent(row16_max(tm), 14), bv = base_exponent(row16_max(tv), 30);
-    const float low = __uint_as_float((bm << 23) + (1u << 20)), low16 = low * 0x1p-16f;
-    const uint32_t word = mix32(((uint32_t)tile * (TILE_ELEMS / 8) + threadIdx.x) ^ key);
-    uint32_t o[4] = {0, 0, 0, 0};
+    const uint32_t word = mix32(((uint32_t)tile * (TILE_ELEMS / 8) + (threadIdx.x >> 1)) ^ key);
+    uint32_t bm, bv, o[2];
+    if (__ballot(max(tm, tv) >= 0x7F800000u) == 0) {
+        bm = base_exponent(half_max(tm), 14);
+        bv = base_exponent(half_max(tv), 30);
+        encode4<false>(m, v, bm, bv, word, o);
+    } else {                                    // the largest FINITE values say the base
+        tm = tv = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t r = word * lane_word(j), um = r & 0xFFFFu, uv = r >> 16;
-        const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-        const float a = __uint_as_float(mb);
-        uint32_t mc = ((mb + (um << 4) + 8u) >> 20) - (bm << 3);
-        if (a < low) mc = a > low16 * ((float)um + 0.5f) ? 1u : 0u;
-        if (mc != 0u) mc |= __float_as_uint(m[j]) >> 31 << 7;
-        if (mb >= 0x7F800000u) mc = 127u;
-        int vs = (int)((vb + (uv << 4) + 8u) >> 20) - (int)(bv << 3);
-        uint32_t vc = vb == 0u ? 0u : (uint32_t)(vs < 1 ? 1 : vs);
-        if (vb >= 0x7F800000u) vc = 255u;
-        o[j >> 1] |= (mc | vc << 8) << (16 * (j & 1));
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+            if ((FULL || j < nv) && mb < 0x7F800000u) tm = max(tm, mb);
+            if ((FULL || j < nv) && vb < 0x7F800000u) tv = max(tv, vb);
+        }
+        bm = base_exponent(half_max(tm), 14);
+        bv = base_exponent(half_max(tv), 30);
+        encode4<true>(m, v, bm, bv, word, o);
     }
-    store_codes<FULL>(e.s0, at, nv, o);
-    if ((threadIdx.x & 15) == 0 && (FULL || nv > 0)) ((uint16_t*)e.s1)[block] = (uint16_t)(bm | bv << 8);
+    store_codes<FULL, NT>(e.s0, at, nv, o);
+    if ((threadIdx.x & 31) == 0 && (FULL || nv > 0)) ((uint16_t*)e.s1)[block] = (uint16_t)(bm | bv << 8);
 }
 
-// One launch: grid-stride over the tiles of up to 40 tensors.  DEV: step count and learning rates come from device memory (a captured graph replays them).
-template <bool Q8, bool DEV, bool MASKED>
-__global__ __launch_bounds__(256) void adamw_step_kernel(StepTable t, StepHyper h) {
-    double inv_bc1 = h.inv_bc1;
-    float ibc2 = h.inv_bc2_sqrt;
+// 1 - b^t on the device: 2^(t log2 b) by the series of e^y, |y| <= ln(2) / 2, whose first term left out is y^13 / 13! < 2^-52
+__device__ __forceinline__ double one_minus_power(double log2_b, int t) {
+    const double x = fmax((double)t * log2_b, -1000.0), n = rint(x), y = (x - n) * 0.693147180559945309417;
+    double s = 1.0 / 479001600.0;
+    constexpr double c[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+#pragma unroll
+    for (int k = 11; k >= 0; --k) s = __builtin_fma(s, y, c[k]);
+    return 1.0 - ldexp(s, (int)n);
+}
+
+// One workgroup, one wave, 256 elements, no loop: the launch hands the tiles out in order and the streams stay local in DRAM.  DEV: step count and learning rates come from
+// device memory (a captured graph replays them).
+template <bool Q8, bool DEV, bool MASKED, bool NT>
+__global__ __launch_bounds__(64) void adamw_step_kernel(StepTable t, StepHyper h) {
+    const uint32_t tile = blockIdx.x;
+    const StepEntry e = t.e[find_tensor(t.first, tile)];
+    float clip = 1.f;
+    if (h.clip) clip = *h.clip;
+    const uint32_t mine = tile - e.first;
     int step = h.step;
+    Fold f = {h.b1, h.omb1, h.b2, h.omb2, h.eps, h.inv_bc2_sqrt, e.decay, e.step_size, clip};
+    at_hand(e.p); at_hand(e.g); at_hand(e.s0); at_hand(e.s1); at_hand(e.master); at_hand(e.numel); at_hand((int)e.kind); at_hand(mine); at_hand(f.decay); at_hand(f.step_size);
+    at_hand(f.b1); at_hand(f.omb1); at_hand(f.b2); at_hand(f.omb2); at_hand(f.eps); at_hand(f.ibc2); at_hand(clip);
+    long long numel = e.numel;
     if (DEV) {
         if (h.guard_count && *h.guard_count > h.guard_limit) return;      // the iteration that made these gradients is void: nothing moves
-        __shared__ double s_bc1;
-        __shared__ float s_bc2;
+        if (h.live_rows && e.row_width > 0) numel = min(numel, (long long)*h.live_rows * e.row_width);     // rows behind the live count are not parameters
         step += *h.step_dev;
-        if (threadIdx.x == 0) {
-            s_bc1 = 1.0 / (1.0 - pow(h.db1, (double)step));
-            s_bc2 = (float)(1.0 / sqrt(1.0 - pow(h.db2, (double)step)));
-        }
-        __syncthreads();
-        inv_bc1 = s_bc1;
-        ibc2 = s_bc2;
+        const double lr = h.lr_dev[e.src], bc = one_minus_power(threadIdx.x & 1 ? h.log2_b2 : h.log2_b1, step);      // both powers in one evaluation
+        const float bcf = (float)bc, bc1 = __shfl(bcf, 0, 64), bc2 = __shfl(bcf, 1, 64);
+        f.ibc2 = 1.f / sqrtf(bc2);
+        f.decay = (float)(1.0 - lr * e.wd);
+        f.step_size = (float)lr / bc1;
     }
-    const float clip = h.clip ? *h.clip : 1.f;
-    for (uint32_t tile = blockIdx.x; tile < h.tiles; tile += gridDim.x) {
-        const int k = __builtin_amdgcn_readfirstlane(find_tensor(t.first, tile));
-        const StepEntry& e = t.e[k];
-        const uint32_t mine = tile - t.first[k];
-        long long numel = e.numel;
-        if (DEV && h.live_rows && e.row_width > 0) numel = min(numel, (long long)*h.live_rows * e.row_width);   // rows behind the live count are not parameters
-        const long long left = numel - (long long)mine * TILE_ELEMS;
-        if (left <= 0) continue;
-        const double lr = DEV ? h.lr_dev[e.src] : e.lr;
-        const Fold f = {h.b1, h.omb1, h.b2, h.omb2, h.eps, ibc2, (float)(1.0 - lr * e.wd), (float)(lr * inv_bc1), clip};
-        const uint32_t key = Q8 ? mix32(h.seed + (uint32_t)step * 0x9E3779B1u + (uint32_t)e.place * 0x85EBCA6Bu) : 0u;
-        const bool full = left >= TILE_ELEMS;
-#define GSICP_STEP(DT, MASTER)                                                                                                             \
-    (full ? step_tile<Q8, DT, MASTER, true, MASKED>(e, f, h.row_freeze, h.grad_rows, key, mine, numel)                                      \
-          : step_tile<Q8, DT, MASTER, false, MASKED>(e, f, h.row_freeze, h.grad_rows, key, mine, numel))
-        if (MASKED || e.kind == F32) GSICP_STEP(F32, false);
-        else if (e.kind == BF16) GSICP_STEP(BF16, false);
-        else if (e.kind == F16) GSICP_STEP(F16, false);
-        else if (e.kind == (BF16 | 4)) GSICP_STEP(BF16, true);
-        else GSICP_STEP(F16, true);
+    const long long left = numel - (long long)mine * TILE_ELEMS;
+    if (left <= 0) return;
+    const uint32_t key = Q8 ? mix32(h.seed + (uint32_t)step * 0x9E3779B1u + (uint32_t)e.place * 0x85EBCA6Bu) : 0u;
+    const bool full = left >= TILE_ELEMS;
+#define GSICP_STEP(DT, MASTER)                                                                                                                    (full ? step_tile<Q8, DT, MASTER, true, MASKED, NT>(e, f, h.row_freeze, h.grad_rows, key, mine, numel)                                               : step_tile<Q8, DT, MASTER, false, MASKED, NT>(e, f, h.row_freeze, h.grad_rows, key, mine, numel))
+    if (MASKED || e.kind == F32) GSICP_STEP(F32, false);
+    else if (e.kind == BF16) GSICP_STEP(BF16, false);
+    else if (e.kind == F16) GSICP_STEP(F16, false);
+    else if (e.kind == (BF16 | 4)) GSICP_STEP(BF16, true);
+    else GSICP_STEP(F16, true);
 #undef GSICP_STEP
-    }
 }
 
 __global__ void adamw_bump_kernel(int* step_dev, const uint32_t* guard_count, uint32_t guard_limit, uint32_t* skipped) {
@@ -366,34 +437,38 @@ __global__ void adamw_bump_kernel(int* step_dev, const uint32_t* guard_count, ui
 struct DecodeEntry { const void* codes; const void* exps; void* m; void* v; long long numel; };
 struct DecodeTable { uint32_t first[64]; DecodeEntry e[64]; };
 
-template <int DT, bool FULL>
+constexpr int DECODE_ELEMS = 2048;     // 256 lanes x 8: with 6 or 10 bytes an element, tiles of one wave are bound by the rate at which workgroups start
+
+template <int DT, bool FULL, bool NT>
 __device__ __forceinline__ void decode_tile(const DecodeEntry& e, uint32_t tile) {
-    const long long at = (long long)tile * TILE_ELEMS + 8 * threadIdx.x;
-    const int nv = FULL ? 8 : (int)max(0ll, min(8ll, e.numel - at));
-    if (nv == 0) return;
-    uint32_t c[4];
-    load_codes<FULL>(e.codes, at, nv, c);
-    const uint32_t exps = ((const uint16_t*)e.exps)[at / QBLOCK];
-    float m[8], v[8];
+    const long long at = (long long)tile * DECODE_ELEMS + 4 * threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t c16 = c[j >> 1] >> (16 * (j & 1));
-        m[j] = decode_m(c16, (exps & 0xFFu) << 23);
-        v[j] = decode_v(c16, (exps >> 8) << 23);
+    for (int h = 0; h < 2; ++h) {
+        const long long i = at + 1024 * h;
+        const int nv = FULL ? 4 : (int)max(0ll, min(4ll, e.numel - i));
+        if (nv == 0) return;
+        uint32_t c[2];
+        load_codes<FULL, NT>(e.codes, i, nv, c);
+        const uint32_t exps = ((const uint16_t*)e.exps)[i / QBLOCK];
+        float m[4], v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c16 = c[j >> 1] >> (16 * (j & 1));
+            m[j] = decode_m(c16, (exps & 0xFFu) << 23);
+            v[j] = decode_v(c16, (exps >> 8) << 23);
+        }
+        store4<DT, FULL, NT>(e.m, i, nv, m);
+        store4<DT, FULL, NT>(e.v, i, nv, v);
     }
-    store8<DT, FULL>(e.m, at, nv, m);
-    store8<DT, FULL>(e.v, at, nv, v);
 }
 // bf16 holds every code's value exactly (four significant bits, f32's exponents)
-template <int DT>
-__global__ __launch_bounds__(256) void adamw_decode_kernel(DecodeTable t, uint32_t tiles) {
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int k = __builtin_amdgcn_readfirstlane(find_tensor(t.first, tile));
-        const DecodeEntry& e = t.e[k];
-        const uint32_t mine = tile - t.first[k];
-        if (e.numel - (long long)mine * TILE_ELEMS >= TILE_ELEMS) decode_tile<DT, true>(e, mine);
-        else decode_tile<DT, false>(e, mine);
-    }
+template <int DT, bool NT>
+__global__ __launch_bounds__(256) void adamw_decode_kernel(DecodeTable t) {
+    const uint32_t k = find_tensor(t.first, blockIdx.x);
+    const DecodeEntry& e = t.e[k];
+    const uint32_t mine = blockIdx.x - t.first[k];
+    if (e.numel - (long long)mine * DECODE_ELEMS >= DECODE_ELEMS) decode_tile<DT, true, NT>(e, mine);
+    else decode_tile<DT, false, NT>(e, mine);
 }
 
 // ------------------------------------------------------------------------------------------------ global norm
@@ -419,7 +494,7 @@ __device__ __forceinline__ double square_sum16(const u32x4& r) {      // of one 
     return s;
 }
 // `lanes` lanes, four 16-byte loads of each in flight; lane l of load k takes unit k * lanes + l
-template <int DT>
+template <int DT, bool NT>
 __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, int lanes, int lane) {
     constexpr int V = DT == F32 ? 4 : 8;
     const long long at = (long long)tile * (4 * V * lanes), left = e.numel - at;
@@ -428,7 +503,7 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
     if (left >= 4 * V * lanes) {
         u32x4 r[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r[k] = *(const u32x4*)(p + 16 * (size_t)(k * lanes + lane));
+        for (int k = 0; k < 4; ++k) r[k] = get<NT>((const u32x4*)(p + 16 * (size_t)(k * lanes + lane)));
 #pragma unroll
         for (int k = 0; k < 4; ++k) s += square_sum16<DT>(r[k]);
     } else {
@@ -444,11 +519,12 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
     }
     return s;
 }
+template <bool NT>
 __device__ __forceinline__ double norm_any_tile(const NormTable& t, uint32_t tile, int lanes, int lane) {
-    const int k = __builtin_amdgcn_readfirstlane(find_tensor(t.first, tile));
+    const uint32_t k = find_tensor(t.first, tile);
     const NormEntry& e = t.e[k];
     const uint32_t mine = tile - t.first[k];
-    return e.dtype == F32 ? norm_tile<F32>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16>(e, mine, lanes, lane) : norm_tile<F16>(e, mine, lanes, lane);
+    return e.dtype == F32 ? norm_tile<F32, NT>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16, NT>(e, mine, lanes, lane) : norm_tile<F16, NT>(e, mine, lanes, lane);
 }
 template <int WAVES>
 __device__ __forceinline__ double block_sum(double s) {      // complete in thread 0
@@ -471,22 +547,28 @@ __device__ __forceinline__ void norm_results(double sum, double max_norm, float*
     *norm_out = norm;
     if (clip_out) *clip_out = max_norm > 0.0 ? (float)(c > 1.0 ? 1.0 : c) : 1.f;
 }
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_norm_kernel(NormTable t, uint32_t tiles, double* partial) {
     double s = 0.0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile(t, tile, 256, threadIdx.x);
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile<NT>(t, tile, 256, threadIdx.x);
     s = block_sum<4>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, double max_norm, float* norm_out, float* clip_out) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
+    for (int i = threadIdx.x; i < n; i += 4096) {      // four loads in flight
+        double x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = i + 1024 * j < n ? partial[i + 1024 * j] : 0.0;
+        s += (x[0] + x[1]) + (x[2] + x[3]);
+    }
     s = block_sum<16>(s);
     if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
 }
 // few small tensors: one workgroup, a tile per WAVE, no second launch
 __global__ __launch_bounds__(1024) void grad_norm_small_kernel(NormTable t, uint32_t tiles, double max_norm, float* norm_out, float* clip_out) {
     double s = 0.0;
-    for (uint32_t tile = threadIdx.x >> 6; tile < tiles; tile += 16) s += norm_any_tile(t, tile, 64, threadIdx.x & 63);
+    for (uint32_t tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tile < tiles; tile += 16) s += norm_any_tile<false>(t, tile, 64, threadIdx.x & 63);
     s = block_sum<16>(s);
     if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
 }
@@ -495,6 +577,10 @@ __global__ __launch_bounds__(1024) void grad_norm_small_kernel(NormTable t, uint
 int fail(const char* what) { g_last_error = what; return -2; }
 
 size_t dtype_bytes(int dt) { return dt == F32 ? 4 : 2; }
+
+// Non-temporal loads and stores past the 256 MB of the memory-side cache: what a call touches and comes back to is then not there any more (measured both ways below), and lines
+// that only pass through cost write-backs of others.
+bool stream_past_cache(unsigned long long bytes) { const char* e = getenv("NT"); return e ? atoi(e) != 0 : bytes > 320ull << 20; }
 
 // what a call writes must not overlap: a tensor given twice would be updated by two workgroups at once
 bool disjoint(std::vector<std::pair<uintptr_t, uintptr_t>>& r) {
@@ -510,11 +596,11 @@ struct StepCall {
     const long long* numel; const int* dtype; const double* lr; const double* wd; const int* place;
 };
 
-template <bool Q8>
+template <bool Q8, bool NT>
 void launch_step(dim3 grid, bool dev, bool masked, hipStream_t stream, const StepTable& t, const StepHyper& h) {
-    if (!dev) hipLaunchKernelGGL((adamw_step_kernel<Q8, false, false>), grid, dim3(256), 0, stream, t, h);
-    else if (!masked) hipLaunchKernelGGL((adamw_step_kernel<Q8, true, false>), grid, dim3(256), 0, stream, t, h);
-    else hipLaunchKernelGGL((adamw_step_kernel<Q8, true, true>), grid, dim3(256), 0, stream, t, h);
+    if (!dev) hipLaunchKernelGGL((adamw_step_kernel<Q8, false, false, NT>), grid, dim3(64), 0, stream, t, h);
+    else if (!masked) hipLaunchKernelGGL((adamw_step_kernel<Q8, true, false, NT>), grid, dim3(64), 0, stream, t, h);
+    else hipLaunchKernelGGL((adamw_step_kernel<Q8, true, true, NT>), grid, dim3(64), 0, stream, t, h);
 }
 
 template <bool Q8>
@@ -533,6 +619,7 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
     const bool masked = dev && (dev->row_freeze || dev->grad_rows);
     static thread_local std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
     ranges.clear();
+    unsigned long long bytes = 0;
     for (int k = 0; k < c.n; ++k) {
         const long long n = c.numel[k];
         if (n < 0 || n >= (1ll << 35)) return fail("gsicp_adamw_step: a tensor has 0 to 2^35 - 1 elements");
@@ -543,24 +630,27 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
         if (!c.params[k] || !c.grads[k] || !c.s0[k] || !c.s1[k]) return fail("gsicp_adamw_step: null pointer of a tensor that is not empty");
         if (master && dt == F32) return fail("gsicp_adamw_step: an f32 parameter has no master");
         if (masked && (dt != F32 || n >= (1ll << 32))) return fail("gsicp_adamw_step: row masks go with f32 parameters of less than 2^32 elements");
+        bytes += (unsigned long long)n * dtype_bytes(dt);      // the gradient
         auto add = [&](const void* q, size_t bytes) { ranges.emplace_back((uintptr_t)q, (uintptr_t)q + bytes); };
         add(c.params[k], (size_t)n * dtype_bytes(dt));
         if (master) add(master, (size_t)n * 4);
         if (Q8) { add(c.s0[k], (size_t)n * 2); add(c.s1[k], (size_t)((n + QBLOCK - 1) / QBLOCK) * 2); }
         else { add(c.s0[k], (size_t)n * 4); add(c.s1[k], (size_t)n * 4); }
     }
+    for (const auto& r : ranges) bytes += r.second - r.first;
     if (!disjoint(ranges)) return fail("gsicp_adamw_step: two tensors that the step writes overlap (the same one given twice?)");
 
     StepHyper h = {};
+    double inv_bc1 = 1.0;
     h.b1 = (float)b1; h.omb1 = (float)(1.0 - b1); h.b2 = (float)b2; h.omb2 = (float)(1.0 - b2); h.eps = (float)eps;
-    h.db1 = b1; h.db2 = b2; h.clip = clip; h.seed = seed;
+    h.log2_b1 = b1 > 0.0 ? std::log2(b1) : -1e9; h.log2_b2 = b2 > 0.0 ? std::log2(b2) : -1e9; h.clip = clip; h.seed = seed;
     if (dev) {
         h.lr_dev = dev->lr_dev; h.step_dev = dev->step_dev; h.step = dev->bump_step == 2 ? 0 : 1;
         h.guard_count = dev->guard_count; h.guard_limit = dev->guard_limit;
         h.live_rows = dev->live_rows; h.row_freeze = dev->row_freeze; h.grad_rows = dev->grad_rows;
     } else {
         h.step = step;
-        h.inv_bc1 = 1.0 / (1.0 - std::pow(b1, step));
+        inv_bc1 = 1.0 / (1.0 - std::pow(b1, step));
         h.inv_bc2_sqrt = (float)(1.0 / std::sqrt(1.0 - std::pow(b2, step)));
     }
     {
@@ -573,19 +663,21 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
                 if (c.numel[k] == 0) continue;
                 StepEntry& e = t.e[n];
                 e.p = c.params[k]; e.g = c.grads[k]; e.s0 = c.s0[k]; e.s1 = c.s1[k]; e.master = c.masters ? c.masters[k] : nullptr;
-                e.numel = c.numel[k]; e.lr = c.lr ? c.lr[k] : 0.0; e.wd = c.wd[k];
+                e.numel = c.numel[k]; e.wd = c.wd[k]; e.first = (uint32_t)tiles;
+                if (!dev) { e.step_size = (float)(c.lr[k] * inv_bc1); e.decay = (float)(1.0 - c.lr[k] * e.wd); }
                 e.row_width = dev && dev->row_width ? dev->row_width[k] : 0;
                 e.kind = (uint16_t)(c.dtype[k] | (e.master ? 4 : 0));
                 e.frozen = (uint16_t)(dev && dev->row_freeze && dev->group_frozen[k] && e.row_width > 0);
                 e.src = k; e.place = c.place ? c.place[k] : k;
                 t.first[n++] = (uint32_t)tiles;
                 tiles += tiles_of(e.numel);
-                if (tiles > 0xF0000000ull) return fail("gsicp_adamw_step: too many elements in one call");
+                if (tiles >= LAST) return fail("gsicp_adamw_step: too many elements in one call");
             }
-            for (int i = n; i < 64; ++i) t.first[i] = 0xFFFFFFFFu;
+            for (int i = n; i < 64; ++i) t.first[i] = LAST;
             if (n == 0) break;
-            h.tiles = (uint32_t)tiles;
-            launch_step<Q8>(dim3((unsigned)std::min<unsigned long long>(tiles, STEP_GRID)), dev != nullptr, masked, stream, t, h);
+            const dim3 grid((unsigned)tiles);
+            if (stream_past_cache(bytes)) launch_step<Q8, true>(grid, dev != nullptr, masked, stream, t, h);
+            else launch_step<Q8, false>(grid, dev != nullptr, masked, stream, t, h);
         }
         if (dev && dev->bump_step == 1)
             hipLaunchKernelGGL(adamw_bump_kernel, dim3(1), dim3(1), 0, stream, dev->step_dev, dev->guard_count, dev->guard_limit, dev->skipped);
@@ -624,9 +716,11 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
     hipStream_t stream = (hipStream_t)stream_v;
     if (n < 0 || (n > 0 && (!moments || !block_exps || !exp_avg || !exp_avg_sq || !numel))) return fail("gsicp_adamw_decode: missing arrays");
     if (dtype != F32 && dtype != BF16) return fail("gsicp_adamw_decode: dtype is 0 (f32) or 1 (bf16)");
+    unsigned long long bytes = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || numel[k] >= (1ll << 35)) return fail("gsicp_adamw_decode: a tensor has 0 to 2^35 - 1 elements");
         if (numel[k] > 0 && (!moments[k] || !block_exps[k] || !exp_avg[k] || !exp_avg_sq[k])) return fail("gsicp_adamw_decode: null pointer of a tensor that is not empty");
+        bytes += (unsigned long long)numel[k] * (dtype == F32 ? 10 : 6);
     }
     for (int k = 0; k < n;) {
         DecodeTable t = {};
@@ -636,14 +730,17 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
             if (numel[k] == 0) continue;
             t.e[m] = {moments[k], block_exps[k], exp_avg[k], exp_avg_sq[k], numel[k]};
             t.first[m++] = (uint32_t)tiles;
-            tiles += tiles_of(numel[k]);
-            if (tiles > 0xF0000000ull) return fail("gsicp_adamw_decode: too many elements in one call");
+            tiles += (unsigned long long)((numel[k] + DECODE_ELEMS - 1) / DECODE_ELEMS);
+            if (tiles >= LAST) return fail("gsicp_adamw_decode: too many elements in one call");
         }
-        for (int i = m; i < 64; ++i) t.first[i] = 0xFFFFFFFFu;
+        for (int i = m; i < 64; ++i) t.first[i] = LAST;
         if (m == 0) break;
-        const dim3 grid((unsigned)std::min<unsigned long long>(tiles, STEP_GRID));
-        if (dtype == F32) hipLaunchKernelGGL((adamw_decode_kernel<F32>), grid, dim3(256), 0, stream, t, (uint32_t)tiles);
-        else hipLaunchKernelGGL((adamw_decode_kernel<BF16>), grid, dim3(256), 0, stream, t, (uint32_t)tiles);
+        const dim3 grid((unsigned)tiles);
+        const bool nt = stream_past_cache(bytes);
+        if (dtype == F32 && nt) hipLaunchKernelGGL((adamw_decode_kernel<F32, true>), grid, dim3(256), 0, stream, t);
+        else if (dtype == F32) hipLaunchKernelGGL((adamw_decode_kernel<F32, false>), grid, dim3(256), 0, stream, t);
+        else if (nt) hipLaunchKernelGGL((adamw_decode_kernel<BF16, true>), grid, dim3(256), 0, stream, t);
+        else hipLaunchKernelGGL((adamw_decode_kernel<BF16, false>), grid, dim3(256), 0, stream, t);
     }
     if (hipGetLastError() != hipSuccess) { g_last_error = "gsicp_adamw_decode: kernel launch failed"; return -1; }
     return 0;
@@ -655,13 +752,14 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
                     void* stream_v) {
     hipStream_t stream = (hipStream_t)stream_v;
     if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !norm_out || !scratch) return fail("gsicp_grad_norm: missing arrays");
-    unsigned long long small = 0;
+    unsigned long long small = 0, bytes = 0;
     int used_tensors = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || numel[k] >= (1ll << 35)) return fail("gsicp_grad_norm: a tensor has 0 to 2^35 - 1 elements");
         if (numel[k] == 0) continue;
         if (!grads[k] || dtype[k] < F32 || dtype[k] > F16) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
         ++used_tensors;
+        bytes += (unsigned long long)numel[k] * dtype_bytes(dtype[k]);
         const int te = norm_tile_elems(dtype[k], 64 * 64);
         small += (unsigned long long)((numel[k] + te - 1) / te);
     }
@@ -679,16 +777,17 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
             t.first[m++] = (uint32_t)tiles;
             const int te = norm_tile_elems(dtype[k], tile_bytes);
             tiles += (unsigned long long)((numel[k] + te - 1) / te);
-            if (tiles > 0xF0000000ull) return fail("gsicp_grad_norm: too many elements in one call");
+            if (tiles >= LAST) return fail("gsicp_grad_norm: too many elements in one call");
         }
-        for (int i = m; i < 64; ++i) t.first[i] = 0xFFFFFFFFu;
+        for (int i = m; i < 64; ++i) t.first[i] = LAST;
         if (one) {
             hipLaunchKernelGGL(grad_norm_small_kernel, dim3(1), dim3(1024), 0, stream, t, (uint32_t)tiles, max_norm, norm_out, clip_out);
             break;
         }
         if (m == 0) break;
         const unsigned grid = (unsigned)std::min<unsigned long long>(tiles, NORM_GRID);
-        hipLaunchKernelGGL(grad_norm_kernel, dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
+        if (stream_past_cache(bytes)) hipLaunchKernelGGL((grad_norm_kernel<true>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
+        else hipLaunchKernelGGL((grad_norm_kernel<false>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
         used += (int)grid;
     }
     if (!one) hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, stream, (const double*)partial, used, max_norm, norm_out, clip_out);

@@ -39,7 +39,7 @@ def decode(moments, exps, dtype=np.float64):
 
     def value(code, base):
         return np.where(code > 0, np.ldexp(1.0 + (code % 8) / 8.0, code // 8 + base - 127), 0.0)
-    m = np.where(mag == 127, np.nan, value(mag, e & 255) * np.where(c & 128, -1.0, 1.0))
+    m = np.where(mag == 127, np.nan, np.where(mag == 0, 0.0, value(mag, e & 255) * np.where(c & 128, -1.0, 1.0)))
     v = np.where(vc == 255, np.inf, value(vc, e >> 8))
     return m.astype(dtype), v.astype(dtype)
 
@@ -56,7 +56,7 @@ def encode(m, v, um, uv):
     low = ((bm << 23) + (1 << 20)).astype(np.uint32).view(np.float32)
     rounded = ((mb + (um << 4) + 8) >> 20) - (bm << 3)
     mc = np.where(a < low, (a > (low * np.float32(2.0 ** -16)) * (um.astype(np.float32) + np.float32(0.5))).astype(np.int64), rounded)
-    mc = np.where(mb >= 0x7F800000, 127, np.where(mc > 0, mc | sign << 7, 0))
+    mc = np.where(mb >= 0x7F800000, 127, mc | sign << 7)                # a zero may carry a sign: it stands for zero all the same
     vc = np.maximum(((vb + (uv << 4) + 8) >> 20) - (bv << 3), 1)
     vc = np.where(vb == 0, 0, np.where(vb >= 0x7F800000, 255, vc))
     return (mc | vc << 8).reshape(-1)[:n].astype(np.uint16), (bm | bv << 8).reshape(-1).astype(np.uint16)
@@ -87,9 +87,10 @@ def step64(p, m, v, g, lr, wd, betas, eps, t, clip=1.0):
         v1 = a + b
         dv = 2 * u * a + (3 * u + 2 * ug) * b + u * v1
         den = np.sqrt(v1) / np.sqrt(1 - b2 ** t) + eps
-        dden = (np.sqrt(v1) / np.sqrt(1 - b2 ** t)) * (0.5 * np.where(v1 > 0, dv / np.where(v1 > 0, v1, 1), 0) + 3 * u) + u * eps + u * den      # root, constant, product; eps; sum
+        dden = (np.sqrt(v1) / np.sqrt(1 - b2 ** t)) * (0.5 * np.where(v1 > 0, dv / np.where(v1 > 0, v1, 1), 0) + 3 * u) + u * eps + u * den      # root (2 u), constant; eps; sum
         upd = lr / (1 - b1 ** t) * m1 / den
-        dupd = np.abs(upd) * (3 * u + dden / den) + lr / (1 - b1 ** t) * dm / den   # step size, quotient, product
+        # step size (a constant), reciprocal (within one unit of its last place: 2 u), product; the sum of den within the root's 2 u, its constant and the sum itself
+        dupd = np.abs(upd) * (4 * u + dden / den) + lr / (1 - b1 ** t) * dm / den
         p1 = p * (1 - lr * wd) - upd
         dp = 2 * u * np.abs(p) + dupd + u * np.abs(p1)
     tiny = 2.0 ** -149

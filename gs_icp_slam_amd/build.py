@@ -93,13 +93,14 @@ def build_tensor_lists(force=False, verbose=True):
     import sysconfig
     import torch
     from torch.utils import cpp_extension
+    rocm_inc = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")
     src = os.path.join(CSRC, "tensor_lists.cpp")
     out = os.path.join(HERE, "_tensor_lists" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
     if force or _newer(out, [src]):
         tl = _torch_lib_dir()
         cmd = (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wno-deprecated-declarations", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{p}" for p in cpp_extension.include_paths()] +
-               [f"-I{sysconfig.get_paths()['include']}", src, "-o", out, f"-L{tl}", f"-Wl,-rpath,{tl}", "-lc10", "-ltorch_cpu", "-ltorch_python"])
+               [f"-I{rocm_inc}", f"-I{sysconfig.get_paths()['include']}", src, "-o", out, f"-L{tl}", f"-Wl,-rpath,{tl}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"])
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)

@@ -36,8 +36,8 @@ extern thread_local std::string g_last_error;
 
 namespace {
 
-constexpr int TABLE = 40;             // tensors per launch: the table travels in the kernel arguments (< 4 KB), nothing is copied or kept
-constexpr int NORM_TABLE = 64;
+constexpr int TABLE = 64;             // tensors per launch: the table travels in the kernel arguments (< 4 KB), nothing is copied or kept
+constexpr int DEV_TABLE = 56;         // with what the device form adds
 constexpr uint32_t LAST = 0x7FFFFFFF; // a tile number that no launch reaches
 constexpr int TILE_ELEMS = 256;       // elements of a workgroup of the step and of the decoding: ONE wave, four consecutive elements a lane, no loop
 constexpr int NORM_GRID = 2048;       // partial sums of one norm launch
@@ -57,18 +57,25 @@ struct StepEntry {
     void* s0;              // exp_avg, or the packed 8-bit moments
     void* s1;              // exp_avg_sq, or the base exponents
     float* master;
-    long long numel;
-    float step_size, decay;     // lr / (1 - b1^t) and 1 - lr wd   (host form)
-    double wd;                  // the device form takes lr from memory
-    uint32_t first;             // its first tile
-    int row_width;         // elements per map row (live rows, masks); 0: whole tensor
-    uint16_t kind;         // Dtype | 4 with a master
-    uint16_t frozen;       // rows with a non-zero freeze word are left alone
-    int src, place;        // index in the caller's arrays (device learning rates), place in the list (random bits)
+    uint64_t word;         // 35 bits numel, 3 bits Dtype | 4 with a master, 1 bit: frozen rows are left alone, 24 bits from 40: place in the list (random bits)
+    union {
+        float scale[2];    // lr / (1 - b1^t) and 1 - lr wd    (host form)
+        double wd;         // the device form takes lr from memory
+    };
+    __host__ __device__ long long numel() const { return (long long)(word & ((1ull << 35) - 1)); }
+    __host__ __device__ uint32_t kind() const { return (uint32_t)(word >> 35) & 7u; }
+    __host__ __device__ bool frozen() const { return (word >> 38 & 1u) != 0; }
+    __host__ __device__ uint32_t place() const { return (uint32_t)(word >> 40); }
 };
-struct StepTable {
-    uint32_t first[64];    // first tile of each tensor; LAST behind them
+template <bool DEV> struct StepTable;
+template <> struct StepTable<false> {
+    uint32_t first[64];    // first tile of each tensor (an empty one has its successor's); LAST behind them
     StepEntry e[TABLE];
+};
+template <> struct StepTable<true> {
+    uint32_t first[64];
+    StepEntry e[DEV_TABLE];
+    int row_width[DEV_TABLE];   // elements per map row (live rows, masks); 0: whole tensor
 };
 struct StepHyper {
     float b1, omb1, b2, omb2, eps;
@@ -82,8 +89,9 @@ struct StepHyper {
     const uint32_t* guard_count;
     uint32_t guard_limit;
     const int *live_rows, *row_freeze, *grad_rows;
+    int src;               // index of the table's first tensor in lr_dev
 };
-static_assert(sizeof(StepTable) + sizeof(StepHyper) <= 4096, "kernel arguments of a launch");
+static_assert(sizeof(StepTable<false>) + sizeof(StepHyper) <= 4096 && sizeof(StepTable<true>) + sizeof(StepHyper) <= 4096, "kernel arguments of a launch");
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x = (x ^ (x >> 16)) * 0x7FEB352Du;
@@ -291,7 +299,8 @@ __device__ __forceinline__ void encode4(const float m[4], const float v[4], uint
 }
 
 template <bool Q8, int DT, bool MASTER, bool FULL, bool MASKED, bool NT>
-__device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, const int* row_freeze, const int* grad_rows, uint32_t key, uint32_t tile, long long numel) {
+__device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, uint32_t row_width, const int* row_freeze, const int* grad_rows, uint32_t key, uint32_t tile,
+                                          long long numel) {
     const long long at = (long long)tile * TILE_ELEMS + 4 * threadIdx.x;
     const int nv = FULL ? 4 : (int)max(0ll, min(4ll, numel - at));
     float p[4], g[4], m[4], v[4];
@@ -308,14 +317,14 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
     }
     uint32_t keep = 0;                          // elements of frozen rows
     if (MASKED) {
-        const uint32_t w = (uint32_t)e.row_width;
+        const uint32_t w = row_width;
         if (w && nv > 0) {
             uint32_t row = (uint32_t)at / w, col = (uint32_t)at - row * w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (FULL || j < nv) {
                     if (grad_rows && grad_rows[row] <= 0) g[j] = 0.f;     // whatever the gradient's memory holds there
-                    if (e.frozen && row_freeze[row] != 0) keep |= 1u << j;
+                    if (e.frozen() && row_freeze[row] != 0) keep |= 1u << j;
                 }
                 if (++col == w) { col = 0; ++row; }
             }
@@ -391,22 +400,23 @@ __device__ __forceinline__ double one_minus_power(double log2_b, int t) {
 // One workgroup, one wave, 256 elements, no loop: the launch hands the tiles out in order and the streams stay local in DRAM.  DEV: step count and learning rates come from
 // device memory (a captured graph replays them).
 template <bool Q8, bool DEV, bool MASKED, bool NT>
-__global__ __launch_bounds__(64) void adamw_step_kernel(StepTable t, StepHyper h) {
-    const uint32_t tile = blockIdx.x;
-    const StepEntry e = t.e[find_tensor(t.first, tile)];
+__global__ __launch_bounds__(64) void adamw_step_kernel(StepTable<DEV> t, StepHyper h) {
+    const uint32_t tile = blockIdx.x, k = find_tensor(t.first, tile), mine = tile - t.first[k];
+    const StepEntry e = t.e[k];
     float clip = 1.f;
     if (h.clip) clip = *h.clip;
-    const uint32_t mine = tile - e.first;
     int step = h.step;
-    Fold f = {h.b1, h.omb1, h.b2, h.omb2, h.eps, h.inv_bc2_sqrt, e.decay, e.step_size, clip};
-    at_hand(e.p); at_hand(e.g); at_hand(e.s0); at_hand(e.s1); at_hand(e.master); at_hand(e.numel); at_hand((int)e.kind); at_hand(mine); at_hand(f.decay); at_hand(f.step_size);
+    Fold f = {h.b1, h.omb1, h.b2, h.omb2, h.eps, h.inv_bc2_sqrt, e.scale[1], e.scale[0], clip};
+    at_hand(e.p); at_hand(e.g); at_hand(e.s0); at_hand(e.s1); at_hand(e.master); at_hand(e.word); at_hand(mine); at_hand(f.decay); at_hand(f.step_size);
     at_hand(f.b1); at_hand(f.omb1); at_hand(f.b2); at_hand(f.omb2); at_hand(f.eps); at_hand(f.ibc2); at_hand(clip);
-    long long numel = e.numel;
-    if (DEV) {
+    long long numel = e.numel();
+    uint32_t row_width = 0;
+    if constexpr (DEV) {
         if (h.guard_count && *h.guard_count > h.guard_limit) return;      // the iteration that made these gradients is void: nothing moves
-        if (h.live_rows && e.row_width > 0) numel = min(numel, (long long)*h.live_rows * e.row_width);     // rows behind the live count are not parameters
+        row_width = (uint32_t)t.row_width[k];
+        if (h.live_rows && row_width > 0) numel = min(numel, (long long)*h.live_rows * row_width);     // rows behind the live count are not parameters
         step += *h.step_dev;
-        const double lr = h.lr_dev[e.src], bc = one_minus_power(threadIdx.x & 1 ? h.log2_b2 : h.log2_b1, step);      // both powers in one evaluation
+        const double lr = h.lr_dev[h.src + k], bc = one_minus_power(threadIdx.x & 1 ? h.log2_b2 : h.log2_b1, step);      // both powers in one evaluation
         const float bcf = (float)bc, bc1 = __shfl(bcf, 0, 64), bc2 = __shfl(bcf, 1, 64);
         f.ibc2 = 1.f / sqrtf(bc2);
         f.decay = (float)(1.0 - lr * e.wd);
@@ -414,13 +424,16 @@ __global__ __launch_bounds__(64) void adamw_step_kernel(StepTable t, StepHyper h
     }
     const long long left = numel - (long long)mine * TILE_ELEMS;
     if (left <= 0) return;
-    const uint32_t key = Q8 ? mix32(h.seed + (uint32_t)step * 0x9E3779B1u + (uint32_t)e.place * 0x85EBCA6Bu) : 0u;
+    const uint32_t key = Q8 ? mix32(h.seed + (uint32_t)step * 0x9E3779B1u + e.place() * 0x85EBCA6Bu) : 0u;
     const bool full = left >= TILE_ELEMS;
-#define GSICP_STEP(DT, MASTER)                                                                                                                    (full ? step_tile<Q8, DT, MASTER, true, MASKED, NT>(e, f, h.row_freeze, h.grad_rows, key, mine, numel)                                               : step_tile<Q8, DT, MASTER, false, MASKED, NT>(e, f, h.row_freeze, h.grad_rows, key, mine, numel))
-    if (MASKED || e.kind == F32) GSICP_STEP(F32, false);
-    else if (e.kind == BF16) GSICP_STEP(BF16, false);
-    else if (e.kind == F16) GSICP_STEP(F16, false);
-    else if (e.kind == (BF16 | 4)) GSICP_STEP(BF16, true);
+    const uint32_t kind = e.kind();
+#define GSICP_STEP(DT, MASTER)                                                                                                                \
+    (full ? step_tile<Q8, DT, MASTER, true, MASKED, NT>(e, f, row_width, h.row_freeze, h.grad_rows, key, mine, numel)                          \
+          : step_tile<Q8, DT, MASTER, false, MASKED, NT>(e, f, row_width, h.row_freeze, h.grad_rows, key, mine, numel))
+    if (MASKED || kind == F32) GSICP_STEP(F32, false);
+    else if (kind == BF16) GSICP_STEP(BF16, false);
+    else if (kind == F16) GSICP_STEP(F16, false);
+    else if (kind == (BF16 | 4)) GSICP_STEP(BF16, true);
     else GSICP_STEP(F16, true);
 #undef GSICP_STEP
 }
@@ -475,7 +488,7 @@ __global__ __launch_bounds__(256) void adamw_decode_kernel(DecodeTable t) {
 // Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split, and the squares of large
 // or small f32 gradients would leave its range.  The sums are split over the workgroups by position alone and joined in a fixed order.
 struct NormEntry { const void* g; long long numel; int dtype, pad; };
-struct NormTable { uint32_t first[64]; NormEntry e[NORM_TABLE]; };
+struct NormTable { uint32_t first[64]; NormEntry e[TABLE]; };
 
 __host__ __device__ constexpr int norm_tile_elems(int dtype, int bytes) { return bytes / (dtype == F32 ? 4 : 2); }
 
@@ -507,14 +520,12 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
 #pragma unroll
         for (int k = 0; k < 4; ++k) s += square_sum16<DT>(r[k]);
     } else {
-        for (int k = 0; k < 4; ++k) {
-            const long long u = (long long)(k * lanes + lane) * V;
-            if (u + V <= left) s += square_sum16<DT>(*(const u32x4*)(p + u * (16 / V)));
-            else
-                for (long long j = u; j < left && j < u + V; ++j) {
-                    const double x = DT == F32 ? ((const float*)p)[j] : from16(((const uint16_t*)p)[j], DT);
-                    s = __builtin_fma(x, x, s);
-                }
+        const int whole = (int)(left / V), rest = (int)(left - (long long)whole * V);
+        for (int u = lane; u < whole; u += lanes) s += square_sum16<DT>(*(const u32x4*)(p + 16 * (size_t)u));
+        if (lane < rest) {
+            const size_t i = (size_t)whole * V + lane;
+            const double x = DT == F32 ? ((const float*)p)[i] : from16(((const uint16_t*)p)[i], DT);
+            s = __builtin_fma(x, x, s);
         }
     }
     return s;
@@ -548,7 +559,7 @@ __device__ __forceinline__ void norm_results(double sum, double max_norm, float*
     if (clip_out) *clip_out = max_norm > 0.0 ? (float)(c > 1.0 ? 1.0 : c) : 1.f;
 }
 template <bool NT>
-__global__ __launch_bounds__(256) void grad_norm_kernel(NormTable t, uint32_t tiles, double* partial) {
+__global__ __launch_bounds__(256, 8) void grad_norm_kernel(NormTable t, uint32_t tiles, double* partial) {
     double s = 0.0;
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile<NT>(t, tile, 256, threadIdx.x);
     s = block_sum<4>(s);
@@ -559,7 +570,9 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __
     for (int i = threadIdx.x; i < n; i += 4096) {      // four loads in flight
         double x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = i + 1024 * j < n ? partial[i + 1024 * j] : 0.0;
+        for (int j = 0; j < 4; ++j) x[j] = partial[min(i + 1024 * j, n - 1)];
+#pragma unroll
+        for (int j = 1; j < 4; ++j) x[j] = i + 1024 * j < n ? x[j] : 0.0;
         s += (x[0] + x[1]) + (x[2] + x[3]);
     }
     s = block_sum<16>(s);
@@ -596,11 +609,44 @@ struct StepCall {
     const long long* numel; const int* dtype; const double* lr; const double* wd; const int* place;
 };
 
-template <bool Q8, bool NT>
-void launch_step(dim3 grid, bool dev, bool masked, hipStream_t stream, const StepTable& t, const StepHyper& h) {
-    if (!dev) hipLaunchKernelGGL((adamw_step_kernel<Q8, false, false, NT>), grid, dim3(64), 0, stream, t, h);
-    else if (!masked) hipLaunchKernelGGL((adamw_step_kernel<Q8, true, false, NT>), grid, dim3(64), 0, stream, t, h);
-    else hipLaunchKernelGGL((adamw_step_kernel<Q8, true, true, NT>), grid, dim3(64), 0, stream, t, h);
+// fills one table from tensor k on and launches it; -> the next tensor, or -1 (too many elements)
+template <bool Q8, bool DEV>
+int launch_step(const StepCall& c, int k, StepHyper& h, double inv_bc1, const gsicp_adamw_device* dev, bool masked, bool nt, hipStream_t stream) {
+    StepTable<DEV> t = {};
+    int n = 0;
+    unsigned long long tiles = 0;
+    h.src = k;
+    for (; k < c.n && n < (DEV ? DEV_TABLE : TABLE); ++k, ++n) {
+        StepEntry& e = t.e[n];
+        e.p = c.params[k]; e.g = c.grads[k]; e.s0 = c.s0[k]; e.s1 = c.s1[k]; e.master = c.masters ? c.masters[k] : nullptr;
+        const uint64_t kind = (uint64_t)c.dtype[k] | (e.master ? 4u : 0u), place = (uint64_t)(c.place ? c.place[k] : k);
+        e.word = (uint64_t)c.numel[k] | kind << 35 | place << 40;
+        if constexpr (DEV) {
+            e.wd = c.wd[k];
+            t.row_width[n] = dev->row_width ? dev->row_width[k] : 0;
+            if (dev->row_freeze && dev->group_frozen[k] && t.row_width[n] > 0) e.word |= 1ull << 38;
+        } else {
+            e.scale[0] = (float)(c.lr[k] * inv_bc1);
+            e.scale[1] = (float)(1.0 - c.lr[k] * c.wd[k]);
+        }
+        t.first[n] = (uint32_t)tiles;
+        tiles += tiles_of(c.numel[k]);
+        if (tiles >= LAST) return -1;
+    }
+    for (int i = n; i < 64; ++i) t.first[i] = LAST;
+    if (tiles == 0) return k;
+    const dim3 grid((unsigned)tiles);
+    if constexpr (!DEV) {
+        if (nt) hipLaunchKernelGGL((adamw_step_kernel<Q8, false, false, true>), grid, dim3(64), 0, stream, t, h);
+        else hipLaunchKernelGGL((adamw_step_kernel<Q8, false, false, false>), grid, dim3(64), 0, stream, t, h);
+    } else if (masked) {
+        if (nt) hipLaunchKernelGGL((adamw_step_kernel<Q8, true, true, true>), grid, dim3(64), 0, stream, t, h);
+        else hipLaunchKernelGGL((adamw_step_kernel<Q8, true, true, false>), grid, dim3(64), 0, stream, t, h);
+    } else {
+        if (nt) hipLaunchKernelGGL((adamw_step_kernel<Q8, true, false, true>), grid, dim3(64), 0, stream, t, h);
+        else hipLaunchKernelGGL((adamw_step_kernel<Q8, true, false, false>), grid, dim3(64), 0, stream, t, h);
+    }
+    return k;
 }
 
 template <bool Q8>
@@ -623,8 +669,9 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
     for (int k = 0; k < c.n; ++k) {
         const long long n = c.numel[k];
         if (n < 0 || n >= (1ll << 35)) return fail("gsicp_adamw_step: a tensor has 0 to 2^35 - 1 elements");
+        const int dt = c.dtype[k], place = c.place ? c.place[k] : k;
+        if (place < 0 || place >= (1 << 24)) return fail("gsicp_adamw_step: a place in the list is 0 to 2^24 - 1");
         if (n == 0) continue;
-        const int dt = c.dtype[k];
         if (dt < F32 || dt > F16) return fail("gsicp_adamw_step: dtype is 0 (f32), 1 (bf16) or 2 (f16)");
         float* master = c.masters ? c.masters[k] : nullptr;
         if (!c.params[k] || !c.grads[k] || !c.s0[k] || !c.s1[k]) return fail("gsicp_adamw_step: null pointer of a tensor that is not empty");
@@ -655,29 +702,10 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
     }
     {
         ProfileScope ps(ST_ADAM, stream);
+        const bool nt = stream_past_cache(bytes);
         for (int k = 0; k < c.n;) {
-            StepTable t = {};
-            int n = 0;
-            unsigned long long tiles = 0;
-            for (; k < c.n && n < TABLE; ++k) {
-                if (c.numel[k] == 0) continue;
-                StepEntry& e = t.e[n];
-                e.p = c.params[k]; e.g = c.grads[k]; e.s0 = c.s0[k]; e.s1 = c.s1[k]; e.master = c.masters ? c.masters[k] : nullptr;
-                e.numel = c.numel[k]; e.wd = c.wd[k]; e.first = (uint32_t)tiles;
-                if (!dev) { e.step_size = (float)(c.lr[k] * inv_bc1); e.decay = (float)(1.0 - c.lr[k] * e.wd); }
-                e.row_width = dev && dev->row_width ? dev->row_width[k] : 0;
-                e.kind = (uint16_t)(c.dtype[k] | (e.master ? 4 : 0));
-                e.frozen = (uint16_t)(dev && dev->row_freeze && dev->group_frozen[k] && e.row_width > 0);
-                e.src = k; e.place = c.place ? c.place[k] : k;
-                t.first[n++] = (uint32_t)tiles;
-                tiles += tiles_of(e.numel);
-                if (tiles >= LAST) return fail("gsicp_adamw_step: too many elements in one call");
-            }
-            for (int i = n; i < 64; ++i) t.first[i] = LAST;
-            if (n == 0) break;
-            const dim3 grid((unsigned)tiles);
-            if (stream_past_cache(bytes)) launch_step<Q8, true>(grid, dev != nullptr, masked, stream, t, h);
-            else launch_step<Q8, false>(grid, dev != nullptr, masked, stream, t, h);
+            k = dev ? launch_step<Q8, true>(c, k, h, inv_bc1, dev, masked, nt, stream) : launch_step<Q8, false>(c, k, h, inv_bc1, dev, masked, nt, stream);
+            if (k < 0) return fail("gsicp_adamw_step: too many elements in one call");
         }
         if (dev && dev->bump_step == 1)
             hipLaunchKernelGGL(adamw_bump_kernel, dim3(1), dim3(1), 0, stream, dev->step_dev, dev->guard_count, dev->guard_limit, dev->skipped);
@@ -746,24 +774,36 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
     return 0;
 }
 
-size_t gsicp_grad_norm_scratch_bytes(int n) { return n <= 0 ? 8 : (size_t)((n + NORM_TABLE - 1) / NORM_TABLE) * NORM_GRID * sizeof(double); }
+// few small tensors, which one workgroup adds up in one launch
+static bool norm_is_small(int n, const long long* numel, const int* dtype) {
+    unsigned long long tiles = 0;
+    int used = 0;
+    for (int k = 0; k < n && used <= TABLE && tiles <= NORM_SMALL_TILES; ++k) {
+        if (numel[k] <= 0) continue;
+        ++used;
+        const int te = norm_tile_elems(dtype[k], 64 * 64);
+        tiles += (unsigned long long)((numel[k] + te - 1) / te);
+    }
+    return used <= TABLE && tiles <= NORM_SMALL_TILES;
+}
+
+size_t gsicp_grad_norm_scratch_bytes(int n, const long long* numel, const int* dtype) {
+    return n <= 0 || !numel || !dtype || norm_is_small(n, numel, dtype) ? 0 : (size_t)((n + TABLE - 1) / TABLE) * NORM_GRID * sizeof(double);
+}
 
 int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
                     void* stream_v) {
     hipStream_t stream = (hipStream_t)stream_v;
-    if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !norm_out || !scratch) return fail("gsicp_grad_norm: missing arrays");
-    unsigned long long small = 0, bytes = 0;
-    int used_tensors = 0;
+    if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !norm_out) return fail("gsicp_grad_norm: missing arrays");
+    unsigned long long bytes = 0;
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || numel[k] >= (1ll << 35)) return fail("gsicp_grad_norm: a tensor has 0 to 2^35 - 1 elements");
         if (numel[k] == 0) continue;
         if (!grads[k] || dtype[k] < F32 || dtype[k] > F16) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
-        ++used_tensors;
         bytes += (unsigned long long)numel[k] * dtype_bytes(dtype[k]);
-        const int te = norm_tile_elems(dtype[k], 64 * 64);
-        small += (unsigned long long)((numel[k] + te - 1) / te);
     }
-    const bool one = used_tensors <= NORM_TABLE && small <= NORM_SMALL_TILES;
+    const bool one = norm_is_small(n, numel, dtype);
+    if (!one && !scratch) return fail("gsicp_grad_norm: missing scratch");
     const int tile_bytes = one ? 64 * 64 : 256 * 64;
     double* partial = (double*)scratch;
     int used = 0;
@@ -771,7 +811,7 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
         NormTable t = {};
         int m = 0;
         unsigned long long tiles = 0;
-        for (; k < n && m < NORM_TABLE; ++k) {
+        for (; k < n && m < TABLE; ++k) {
             if (numel[k] == 0) continue;
             t.e[m] = {grads[k], numel[k], dtype[k], 0};
             t.first[m++] = (uint32_t)tiles;

@@ -2,7 +2,7 @@
 // Host code only.  Why native: a step over a hundred small tensors is bound by the host, and five Python calls per tensor and list (device, dtype, contiguity, size, address;
 // ~0.2 us together) cost more than the kernel; here they are a few loads.
 //
-//   pack(what, names, rules, list, ...) -> (device index, n, address, keep)
+//   pack(what, names, rules, list, ...) -> (device index, whether it is the current one, its current stream, n, address, keep)
 //
 // One rule (a character) and one name (for the errors) per list; the first list has rule 'p' or 'c' and says device, length and element counts:
 //   p  float32 / bfloat16 / float16 (their codes are recorded)      g  the first list's dtype, read only      f  float32         h  int16
@@ -16,6 +16,8 @@
 #include <exception>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 namespace {
@@ -101,7 +103,9 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             }
             if (why) { Py_DECREF(keep); return refuse(what, name, why); }
         }
-        return Py_BuildValue("(inKN)", device, n, (unsigned long long)(uintptr_t)base, keep);
+        const unsigned long long stream = (unsigned long long)(uintptr_t)c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
+        PyObject* current = c10::hip::current_device() == device ? Py_True : Py_False;
+        return Py_BuildValue("(iOKnKN)", device, current, stream, n, (unsigned long long)(uintptr_t)base, keep);
     } catch (const std::exception& e) {
         Py_XDECREF(keep);
         PyErr_SetString(PyExc_RuntimeError, e.what());
@@ -109,7 +113,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
-PyMethodDef methods[] = {{"pack", (PyCFunction)(void (*)(void))pack, METH_FASTCALL, "pack(what, names, rules, list, ...) -> (device index, n, address, keep)"},
+PyMethodDef methods[] = {{"pack", (PyCFunction)(void (*)(void))pack, METH_FASTCALL, "pack(what, names, rules, list, ...) -> (device index, current, stream, n, address, keep)"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", "lists of torch tensors as host arrays of the C ABI", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

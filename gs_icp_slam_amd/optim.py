@@ -13,7 +13,7 @@ is then an int32 device tensor shared by the parameters that were first stepped 
 Beside it, for parameters of any number and of f32, bf16 or f16 (no reference counterpart: the reference trains with torch.optim.Adam):
 
     norm = grad_norm(grads)                                               # 2-norm over all of them, a device scalar
-    adamw_step(params, grads, exp_avgs, exp_avg_sqs, lr=..., step=t)      # torch.optim.AdamW's step, one launch per 40 tensors
+    adamw_step(params, grads, exp_avgs, exp_avg_sqs, lr=..., step=t)      # torch.optim.AdamW's step, one launch per 64 tensors
     adamw_step_8bit(params, grads, moments, block_exps, lr=..., step=t)   # the same with both moments in 8 bits
     exp_avgs, exp_avg_sqs = decode_moments(moments, block_exps)           # what 8-bit moments stand for
 
@@ -259,7 +259,8 @@ _tensor_lists = None
 
 
 def _pack(what, names, rules, *lists):
-    """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, n, [addresses of each list], numels, dtype codes, what keeps them alive)."""
+    """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, whether it is the current one, its current stream, n, address of the arrays, what
+    keeps them alive).  The arrays: n addresses per list, n element counts (8 bytes each), n dtype codes."""
     global _tensor_lists
     if _tensor_lists is None:
         try:
@@ -267,9 +268,7 @@ def _pack(what, names, rules, *lists):
         except ImportError as e:
             raise ImportError("gs_icp_slam_amd/_tensor_lists not found: build it with `python -m gs_icp_slam_amd.build`") from e
         _tensor_lists = module
-    device, n, base, keep = _tensor_lists.pack(what, names, rules, *lists)
-    k = len(lists)
-    return device, n, [base + 8 * n * i for i in range(k)], base + 8 * n * k, base + 8 * n * (k + 1), keep
+    return _tensor_lists.pack(what, names, rules, *lists)
 
 
 def _at(a):
@@ -286,38 +285,39 @@ def _doubles(what, name, value, n):
     return a
 
 
-def _call(fn, name, device, *args):
-    """fn(*args, current stream of `device`) with that device current."""
-    if torch.cuda.current_device() == device:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(name, device, current, *args):
+    """The entry point `name` of the library with `device` current."""
+    fn = getattr(_lib.load(), name)
+    if current:
+        rc = fn(*args)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args)
     if rc < 0:
         _lib.check(rc, name)
 
 
-def _norm(what, device, n, addresses, numels, codes, max_norm):
-    """-> (norm: 0-dim f32 on the device, scratch whose first word is the clip factor)."""
-    if max_norm is None:
-        max_norm = 0.0
-    elif not max_norm > 0.0:
-        raise RuntimeError(f"{what}: max_norm must be positive")
-    lib = _lib.load()
+def _norm(what, device, current, stream, n, addresses, numels, codes, max_norm):
+    """-> (norm: 0-dim f32 on the device, buffer whose first word is the clip factor or None)."""
     dev = torch.device("cuda", device)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    size = int(lib.gsicp_grad_norm_scratch_bytes(n))
-    scratch = torch.empty(size + 8, dtype=torch.uint8, device=dev)
-    at = scratch.data_ptr()
-    _call(lib.gsicp_grad_norm, "gsicp_grad_norm", device, n, addresses, numels, codes, float(max_norm), norm.data_ptr(), at, at + 8)
-    return norm, scratch
+    size = _lib.load().gsicp_grad_norm_scratch_bytes(n, numels, codes)
+    buffer = clip = scratch = None
+    if size or max_norm is not None:
+        if max_norm is not None and not max_norm > 0.0:
+            raise RuntimeError(f"{what}: max_norm must be positive")
+        buffer = torch.empty(size + 8, dtype=torch.uint8, device=dev)
+        clip = buffer.data_ptr()
+        scratch = clip + 8
+    _call("gsicp_grad_norm", device, current, n, addresses, numels, codes, max_norm or 0.0, norm.data_ptr(), clip, scratch, stream)
+    return norm, buffer
 
 
 def grad_norm(tensors):
     """2-norm over all elements of `tensors` (f32, bf16 or f16, mixed, any sizes, contiguous, one device) as a 0-dim f32 tensor on their device; nothing synchronises.
     Squares and sums are taken in double and in a fixed order: the same tensors give the same bits."""
-    device, n, (g,), numels, codes, keep = _pack("grad_norm", ("tensors",), "p", list(tensors))
-    return _norm("grad_norm", device, n, g, numels, codes, None)[0]
+    device, current, stream, n, at, keep = _pack("grad_norm", ("tensors",), "p", tensors)
+    return _norm("grad_norm", device, current, stream, n, at, at + 8 * n, at + 16 * n, None)[0]
 
 
 _NAMES_32, _NAMES_8 = ("parameters", "gradients", "exp_avgs", "exp_avg_sqs"), ("parameters", "gradients", "moments", "block_exps")
@@ -328,31 +328,32 @@ def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, 
     """Checks, lays out and launches a step of either form; -> the norm or None.  clip: device address of a factor taken before (max_norm is then not looked at);
     device_form(): the gsicp_adamw_device of a captured step and what it points to."""
     if masters is None:
-        device, n, (p, g, s0, s1), numels, codes, keep = _pack(what, _NAMES_32 if bits == 32 else _NAMES_8, "pgff" if bits == 32 else "pghb", params, grads, first, second)
-        mast = None
+        device, current, stream, n, at, keep = _pack(what, _NAMES_32 if bits == 32 else _NAMES_8, "pgff" if bits == 32 else "pghb", params, grads, first, second)
+        mast, numels = None, at + 32 * n
     else:
-        device, n, (p, g, s0, s1, mast), numels, codes, keep = _pack(what, _NAMES_32_MASTERS if bits == 32 else _NAMES_8_MASTERS, "pgffm" if bits == 32 else "pghbm",
-                                                                     params, grads, first, second, masters)
+        device, current, stream, n, at, keep = _pack(what, _NAMES_32_MASTERS if bits == 32 else _NAMES_8_MASTERS, "pgffm" if bits == 32 else "pghbm", params, grads, first, second,
+                                                     masters)
+        mast, numels = at + 32 * n, at + 40 * n
+    codes = numels + 8 * n
     weight_decay = _doubles(what, "weight_decay", weight_decay, n)
     if device_form is None:
         lr, dev, dev_keep = _doubles(what, "lr", lr, n), None, None
     else:
         lr, (dev, dev_keep) = None, device_form()
-    norm = scratch = None
+    norm = buffer = None
     if clip is None and max_norm is not None:
-        norm, scratch = _norm(what, device, n, g, numels, codes, max_norm)
-        clip = scratch.data_ptr()
-    lib = _lib.load()
+        norm, buffer = _norm(what, device, current, stream, n, at + 8 * n, numels, codes, max_norm)
+        clip = buffer.data_ptr()
+    args = (n, at, at + 8 * n, mast, at + 16 * n, at + 24 * n, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step))
     if bits == 32:
-        _call(lib.gsicp_adamw_step, "gsicp_adamw_step", device, n, p, g, mast, s0, s1, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step), clip, dev)
+        _call("gsicp_adamw_step", device, current, *args, clip, dev, stream)
     else:
-        _call(lib.gsicp_adamw_step_8bit, "gsicp_adamw_step_8bit", device, n, p, g, mast, s0, s1, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step),
-              int(seed) & 0xFFFFFFFF, _at(place), clip, dev)
+        _call("gsicp_adamw_step_8bit", device, current, *args, int(seed) & 0xFFFFFFFF, _at(place), clip, dev, stream)
     return norm
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr, step, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, masters=None, max_norm=None):
-    """One torch.optim.AdamW step (amsgrad and maximize off) over all `params`, in place; one launch per 40 tensors.
+    """One torch.optim.AdamW step (amsgrad and maximize off) over all `params`, in place; one launch per 64 tensors.
 
     params, grads: lists of contiguous f32 / bf16 / f16 tensors on one device, a gradient of its parameter's dtype; exp_avgs, exp_avg_sqs: f32; masters: list of f32 tensors (or
     None entries) that take the update of 16-bit parameters, which then receive it rounded.  lr, weight_decay: a number, or one per tensor.  step: the 1-based count of this
@@ -386,16 +387,16 @@ def decode_moments(moments, block_exps, dtype=torch.float32):
         return [], []
     if dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError("decode_moments: dtype is float32 or bfloat16")
-    device, n, (c, e), numels, _, keep = _pack("decode_moments", ("moments", "block_exps"), "cb", moments, block_exps)
+    device, current, stream, n, at, keep = _pack("decode_moments", ("moments", "block_exps"), "cb", moments, block_exps)
     exp_avgs = [torch.empty(t.shape, dtype=dtype, device=t.device) for t in moments]
     exp_avg_sqs = [torch.empty(t.shape, dtype=dtype, device=t.device) for t in moments]
     m, v = (array.array("Q", [t.data_ptr() for t in ts]) for ts in (exp_avgs, exp_avg_sqs))
-    _call(_lib.load().gsicp_adamw_decode, "gsicp_adamw_decode", device, n, c, e, _at(m), _at(v), numels, int(dtype == torch.bfloat16))
+    _call("gsicp_adamw_decode", device, current, n, at, at + 8 * n, _at(m), _at(v), at + 16 * n, int(dtype == torch.bfloat16), stream)
     return exp_avgs, exp_avg_sqs
 
 
 class FusedAdamW(FusedAdam):
-    """torch.optim.AdamW (amsgrad and maximize off) over any number of f32, bf16 and f16 parameters, one launch per 40 of them with the same betas, eps and step count.
+    """torch.optim.AdamW (amsgrad and maximize off) over any number of f32, bf16 and f16 parameters, one launch per 64 of them with the same betas, eps and step count.
 
     state_bits      32: state[p] = {"step", "exp_avg", "exp_avg_sq"} (f32; torch's layout, so GaussianStore and the reference's append / prune keep working)
                     8: state[p] = {"step", "moments", "block_exps"} — adamw_step_8bit's; `moments(p)` gives their values.  A map that grows or is pruned needs 32: its rows
@@ -500,15 +501,15 @@ class FusedAdamW(FusedAdam):
                     st["step"] = fresh.setdefault((int(st["step"]), p.device), torch.full((), int(st["step"]), dtype=torch.int32, device=p.device))
                 key = (float(b1), float(b2), float(group["eps"]), st["step"].data_ptr() if self.capturable else int(st["step"]), p.device)
                 buckets.setdefault(key, []).append((p, p.grad.contiguous(), st, gi, pi, place))
-        clip = scratch = None
+        clip = buffer = None
         if self.max_grad_norm is not None and buckets:
             if self._grad_rows is not None:
                 raise RuntimeError("FusedAdamW: max_grad_norm reads every gradient row, set_grad_row_mask says some were not written")
             if len({key[4] for key in buckets}) > 1:
                 raise RuntimeError("FusedAdamW(max_grad_norm): the parameters live on several devices")
-            device, n, (g,), numels, codes, keep = _pack("FusedAdamW", ("gradients",), "p", [t[1] for items in buckets.values() for t in items])
-            self.last_grad_norm, scratch = _norm("FusedAdamW", device, n, g, numels, codes, self.max_grad_norm)
-            clip = scratch.data_ptr()
+            device, current, stream, n, at, keep = _pack("FusedAdamW", ("gradients",), "p", [t[1] for items in buckets.values() for t in items])
+            self.last_grad_norm, buffer = _norm("FusedAdamW", device, current, stream, n, at, at + 8 * n, at + 16 * n, self.max_grad_norm)
+            clip = buffer.data_ptr()
         last_of = {key[3:]: key for key in buckets}         # a device counter is advanced by the last launch that reads it
         first, second = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
         for key, items in buckets.items():

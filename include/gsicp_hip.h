@@ -407,7 +407,7 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
                            const int* group_frozen, const int* grad_rows_dev, void* stream);
 
 /* ---- AdamW over many tensors (no reference counterpart: the reference trains with torch.optim.Adam; these stand beside gsicp_adam_step) ----
- * torch.optim.AdamW's step (amsgrad, maximize off) over any number of tensors, 40 per launch:
+ * torch.optim.AdamW's step (amsgrad, maximize off) over any number of tensors, 64 per launch (56 in the device form):
  *     g' = *clip g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
  *     p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
@@ -446,8 +446,8 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
                        int dtype, void* stream);
 /* *norm_out = 2-norm over all elements of n tensors (dtype[k] as above; squares and sums in double, fixed order), *clip_out (may be NULL) = min(1, max_norm /
  * (norm + 1e-6)) — the factor of torch.nn.utils.clip_grad_norm_ —, or 1 when max_norm <= 0.  norm_out, clip_out: DEVICE; scratch: DEVICE, 8-byte aligned,
- * gsicp_grad_norm_scratch_bytes(n) bytes, needs no initialisation and holds nothing afterwards. */
-size_t gsicp_grad_norm_scratch_bytes(int n);
+ * gsicp_grad_norm_scratch_bytes() bytes (0 for few small tensors: scratch may then be NULL), needs no initialisation and holds nothing afterwards. */
+size_t gsicp_grad_norm_scratch_bytes(int n, const long long* numel, const int* dtype);
 int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
                     void* stream);
 

@@ -13,7 +13,7 @@ from tests.util import make_settings, torch_inputs
 pytestmark = pytest.mark.gpu
 
 SIZES = [0, 1, 2, 7, 8, 9, 16, 63, 127, 128, 129, 255, 256, 1000, 2047, 2048, 2049, 4096, 4097, 5003]
-MANY = (SIZES * 3)[:45]                       # more tensors than one launch takes
+MANY = (SIZES * 4)[:70]                       # more tensors than one launch takes
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
@@ -463,6 +463,28 @@ def test_captured_steps_follow_eager_ones(bits, max_norm):
     b.param_groups[0]["lr"] = a.param_groups[0]["lr"] = 2e-2          # a new learning rate reaches the replays
     b.sync_lr()
     eager_pair(30, graphs[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_device_form_over_more_tensors_than_a_launch_takes(bits):
+    from gs_icp_slam_amd.optim import FusedAdamW
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    ps = [torch.randn(n, device="cuda", generator=gen) for n in [0] + MANY + MANY[:60] + [0]]
+    host, dev = ([torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2))
+    # every third group has a learning rate of its own: each tensor must find its own entry of the device array
+    groups = lambda q: [{"params": q[0::3], "lr": 1e-2}, {"params": q[1::3], "lr": 3e-3, "weight_decay": 0.5}, {"params": q[2::3], "lr": 1e-4}]     # noqa: E731
+    a, b = FusedAdamW(groups(host), state_bits=bits, seed=4), FusedAdamW(groups(dev), state_bits=bits, seed=4, capturable=True)
+    for k in range(3):
+        for p, q in zip(host, dev):
+            q.grad = p.grad = torch.randn(p.shape, device="cuda", generator=gen)
+        a.step()
+        b.step()
+    for p, q in zip(host, dev):
+        if p.numel():
+            # step size and root are a few 2^-24 apart (float32 on the device), every step rounds
+            assert (p - q).abs().max() <= 3 * 2.0 ** -23 * (6 + 10 * 1e-2 * 4)
+            for name in ("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps"):
+                assert torch.equal(a.state[p][name], b.state[q][name])
 
 
 def test_steps_on_another_stream():

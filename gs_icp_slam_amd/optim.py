@@ -358,7 +358,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr, step, betas=(0.9, 0.
     params, grads: lists of contiguous f32 / bf16 / f16 tensors on one device, a gradient of its parameter's dtype; exp_avgs, exp_avg_sqs: f32; masters: list of f32 tensors (or
     None entries) that take the update of 16-bit parameters, which then receive it rounded.  lr, weight_decay: a number, or one per tensor.  step: the 1-based count of this
     step.  max_norm: clip by the global norm of `grads` (torch.nn.utils.clip_grad_norm_'s factor; the gradients themselves stay as they are) — the norm is returned as a 0-dim
-    tensor, else None.  No tensor that the step writes may overlap another."""
+    tensor, else None.  No tensor that the step writes may overlap another.  In a captured graph the replays repeat this step count (FusedAdamW(capturable=True) counts on the
+    device)."""
     params = list(params)
     if not params:
         return None
@@ -433,7 +434,9 @@ class FusedAdamW(FusedAdam):
 
     def moments(self, p):
         """(exp_avg, exp_avg_sq) of a parameter that has been stepped, in f32, whatever state_bits is (a copy with 8, the state itself with 32)."""
-        st = self.state[p]
+        st = self.state.get(p)
+        if not st:
+            raise RuntimeError("FusedAdamW.moments: this parameter has not been stepped")
         if self.state_bits == 32:
             return st["exp_avg"], st["exp_avg_sq"]
         (m,), (v,) = decode_moments([st["moments"]], [st["block_exps"]])
@@ -481,7 +484,7 @@ class FusedAdamW(FusedAdam):
                 loss = closure()
         if step_already_bumped and not self.capturable:
             raise RuntimeError("FusedAdamW.step(step_already_bumped=True) needs capturable=True (a device step counter)")
-        buckets, fresh, place = {}, {}, -1
+        buckets, fresh, place, may_run = {}, {}, -1, self.capturable
         for gi, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             for pi, p in enumerate(group["params"]):
@@ -490,6 +493,10 @@ class FusedAdamW(FusedAdam):
                     continue
                 if not p.is_cuda:
                     raise RuntimeError("FusedAdamW (gfx950): parameters must live on the HIP device; there is no CPU path")
+                if not may_run:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("FusedAdamW: capturing a step needs capturable=True (the replays would repeat one step count)")
+                    may_run = True
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW: sparse gradients are not supported")
                 st = self.state[p]

@@ -411,8 +411,8 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
  *     g' = *clip g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
  *     p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
- * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 is
- * allowed, < 2^35), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap (checked; -2).
+ * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 to
+ * 2^33), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap anything else it is given (checked; -2).
  * clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's clip_out), or NULL.  step: the 1-based count after the increment.
  * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (live_rows and the row masks: f32
  * parameters of < 2^32 elements). */
@@ -434,7 +434,7 @@ int gsicp_adamw_step(int n, void* const* params, const void* const* grads, float
                      const float* clip, const gsicp_adamw_device* dev, void* stream);
 /* The same step with both moments in 8 bits: moments (uint16[numel]: low byte sign and 7-bit code of exp_avg, high byte code of exp_avg_sq) and block_exps
  * (uint16[ceil(numel / 128)]: low / high byte the base exponent of the block's first / second moments).  A code c > 0 with base b is (1 + (c & 7) / 8) *
- * 2^((c >> 3) + b - 127), 0 is zero; code 127 of the first moment is NaN, 255 of the second infinity.  All-zero arrays are the state before the first step.  Moments are
+ * 2^((c >> 3) + b - 127), 0 is zero (whatever its sign bit); code 127 of the first moment is NaN, 255 of the second infinity.  All-zero arrays are the state before the first step.  Moments are
  * rounded stochastically: with mix(x) = { x ^= x >> 16; x *= 0x7FEB352D; x ^= x >> 15; x *= 0x846CA68B; x ^= x >> 16 } and L = the eight odd words of lane_word (adamw.hip),
  * element j of the tensor at place[k] (HOST int[n]; NULL: k) takes the halves of mix((j >> 3) ^ mix(seed + step * 0x9E3779B1 + place * 0x85EBCA6B)) * L[j & 7]: the same
  * seed, step and place give the same bits.  The device form takes no live_rows and no row_freeze. */

@@ -97,13 +97,14 @@ def test_c_abi_refuses_before_it_launches():
     D = _lib.AdamWDevice
     width = (ctypes.c_int * 2)(3, 3)
     for eight in (False, True):
-        assert step(eight=eight, numel=[100, -1]) == -2 and step(eight=eight, numel=[100, 1 << 35]) == -2
+        assert step(eight=eight, numel=[100, -1]) == -2 and step(eight=eight, numel=[100, (1 << 33) + 1]) == -2
         assert step(eight=eight, dtype=[0, 3]) == -2 and step(eight=eight, dtype=[-1, 0]) == -2
         for name in ("params", "grads", "s0", "s1"):
             assert step(eight=eight, **{name: None}) == -2
             assert step(eight=eight, **{name: [4096, 0]}) == -2
         assert step(eight=eight, params=[4096, 4096]) == -2 and step(eight=eight, params=[4096, 4100]) == -2           # the same one, an overlap
         assert step(eight=eight, s0=[4096, 1 << 21]) == -2                                                             # a moment inside a parameter
+        assert step(eight=eight, grads=[4096, 1 << 20]) == -2 and step(eight=eight, grads=[(1 << 21) + 4, 1 << 20]) == -2            # a gradient inside what is written
         assert step(eight=eight, masters=[1 << 23, 0]) == -2                                                           # f32 with a master
         assert step(eight=eight, betas=(1.0, 0.999)) == -2 and step(eight=eight, betas=(0.9, -0.1)) == -2 and step(eight=eight, betas=(float("nan"), 0.9)) == -2
         assert step(eight=eight, eps=-1.0) == -2 and step(eight=eight, eps=float("nan")) == -2
@@ -125,10 +126,10 @@ def test_c_abi_refuses_before_it_launches():
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(0), 0.0, None, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(5), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(0), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
-    assert lib.gsicp_grad_norm(1, one(64), k(1 << 35), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(64), k((1 << 33) + 1), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(1 << 30), (ctypes.c_int * 1)(0), 0.0, 64, 64, None, None) == -2          # a large set needs its scratch
     size = lambda n, each: lib.gsicp_grad_norm_scratch_bytes(n, (ctypes.c_longlong * n)(*[each] * n), (ctypes.c_int * n)(*[0] * n))      # noqa: E731
-    assert size(1, 5) == size(128, 7) == 0 and size(129, 7) > size(1, 1 << 30) > 0
+    assert size(1, 5) == size(64, 7) == 0 and size(65, 7) == size(1, 1 << 30) > 0 and size(129, 7) > size(128, 7)
 
 
 def test_python_layer_has_no_cpu_path_and_refuses_bad_options():

@@ -142,6 +142,12 @@ def test_a_large_tensor_beside_small_ones_over_many_workgroups(bits):
     Case([9, 5_000_011, 1, 700], torch.float32, False, bits, seed=2).step(50)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_set_that_streams_past_the_cache(bits):
+    """More than 128 MiB touched: the non-temporal form of the step, behind a norm of many workgroups."""
+    Case([14_000_003, 77], torch.float32, False, bits, seed=6).step(7, max_norm=1e-2)
+
+
 def test_wide_range_inside_a_block_of_8_bit_moments():
     """Blocks whose values span far more than the codes' exponents, values at the ends of float32, subnormals, zeros of both signs."""
     from gs_icp_slam_amd.optim import adamw_step_8bit
@@ -561,12 +567,12 @@ def test_a_map_that_grows_and_is_pruned(stable, n_rest):
         assert all(not bool(store.view("p", k).isnan().any()) and not bool(store.params[k].isnan().any()) for k in NAMES)
 
 
+@pytest.mark.parametrize("rows", [2777, 700_001])          # the larger one streams past the cache
 @pytest.mark.parametrize("bits", [32, 8])
-def test_row_masks_and_guard_equal_a_step_on_masked_gradients(bits):
+def test_row_masks_and_guard_equal_a_step_on_masked_gradients(bits, rows):
     """Culled rows count as zero gradients whatever the memory holds; frozen rows (32-bit moments) do not move; a tripped guard moves nothing."""
     from gs_icp_slam_amd.optim import FusedAdamW
-    rows = 2777
-    shapes = [(rows, 3), (rows, 1, 3), (rows, 15, 3), (rows, 1), (rows, 4), (rows, 7)]
+    shapes = [(rows, 3), (rows, 1, 3), (rows, 15, 3), (rows, 1), (rows, 4), (rows, 7), (rows, 2), (rows, 0)]
     gen = torch.Generator(device="cuda").manual_seed(8)
     ps = [torch.randn(s, device="cuda", generator=gen) for s in shapes]
     make = lambda: [torch.nn.Parameter(p.clone()) for p in ps]       # noqa: E731
@@ -705,6 +711,7 @@ def test_refusals_on_the_device():
         lambda: adamw_step([z(8)], [z(8)], [z(8)], [z(8)], masters=[z(8)], **ok),                     # an f32 parameter has no master
         lambda: adamw_step_8bit([z(200)], [z(200)], [z(200, dt=torch.int16)], [z(1, dt=torch.int16)], **ok),
         lambda: adamw_step_8bit([z(200)], [z(200)], [z(200)], [z(2, dt=torch.int16)], **ok),
+        lambda: adamw_step([z(8)], [buf[:8]], [buf[4:12]], [z(8)], **ok),                             # a gradient inside a moment
         lambda: decode_moments([z(200, dt=torch.int16)], [z(2, dt=torch.int16)], dtype=torch.float16),
         lambda: grad_norm([]),
         lambda: grad_norm([z(4, dt=torch.int32)]),
@@ -714,7 +721,11 @@ def test_refusals_on_the_device():
             f()
             pytest.fail(f"call {k} was not refused")
     assert adamw_step([], [], [], [], **ok) is None
+    g8 = z(8)
+    adamw_step([z(8), z(8)], [g8, g8], [z(8), z(8)], [z(8), z(8)], **ok)                              # one gradient for two parameters is read twice
     opt = FusedAdamW([torch.nn.Parameter(z(8))], state_bits=8, capturable=True)
+    with pytest.raises(RuntimeError):
+        opt.moments(opt.param_groups[0]["params"][0])
     with pytest.raises(RuntimeError):
         opt.set_live_rows(z(1, dt=torch.int32))
     with pytest.raises(RuntimeError):
@@ -726,7 +737,8 @@ def test_refusals_on_the_device():
     with pytest.raises(RuntimeError):
         opt.step()
     opt.set_grad_row_mask(None)
-    g = torch.cuda.CUDAGraph()
-    with pytest.raises(RuntimeError):
-        with torch.cuda.graph(g):       # the learning rates have no device copy yet
-            opt.step()
+    host = FusedAdamW([p])
+    for o in (opt, host):               # the learning rates have no device copy yet; a step count of the host cannot be replayed
+        with pytest.raises(RuntimeError):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                o.step()

@@ -78,6 +78,7 @@ SIGNATURES = {
     "gsicp_adamw_step": (c_int, [c_int] + [c_void_p] * 9 + [c_double, c_double, c_double, c_int, c_void_p, c_void_p, c_void_p]),
     "gsicp_adamw_step_8bit": (c_int, [c_int] + [c_void_p] * 9 + [c_double, c_double, c_double, c_int, ctypes.c_uint, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gsicp_adamw_decode": (c_int, [c_int] + [c_void_p] * 5 + [c_int, c_void_p]),
+    "gsicp_adamw_gather_rows": (c_int, [c_int] + [c_void_p] * 6 + [ctypes.c_longlong, ctypes.c_longlong, c_void_p]),
     "gsicp_grad_norm_scratch_bytes": (c_size_t, [c_int, c_void_p, c_void_p]),
     "gsicp_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gsicp_stream_create_cu_mask": (c_void_p, [c_int, c_int]),

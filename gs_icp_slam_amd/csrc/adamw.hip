@@ -524,6 +524,47 @@ __global__ __launch_bounds__(256) void adamw_decode_kernel(DecodeTable t) {
     else decode_tile<DT, false, NT>(e, mine);
 }
 
+// ------------------------------------------------------------------------------------------------ rows of 8-bit moments
+// Row r of the result is row index[r] of the source, re-blocked.  As bases are powers of two, a code moves to another base by adding eight times the difference of the bases: exact,
+// but for codes that fall below the new block's smallest (first moments become zero, second the smallest code).  Rows that the source does not have come out zero.
+struct GatherEntry { const uint16_t* codes; const uint16_t* exps; uint16_t* out_codes; uint16_t* out_exps; uint32_t width, magic; };
+struct GatherTable { uint32_t first[64]; GatherEntry e[TABLE]; };
+static_assert(sizeof(GatherTable) + 64 <= 4096, "kernel arguments of a launch");
+
+__global__ __launch_bounds__(64) void adamw_gather_kernel(GatherTable t, const long long* __restrict__ index, uint32_t n_rows, long long src_rows) {
+    const uint32_t k = find_tensor(t.first, blockIdx.x), mine = blockIdx.x - t.first[k];
+    const GatherEntry e = t.e[k];
+    const Rows rows = {e.width, e.magic, e.width > 1u ? 31u - __builtin_clz(e.width - 1u) : 0u, nullptr, nullptr};
+    const uint32_t numel = n_rows * e.width, at = mine * TILE_ELEMS + 4 * threadIdx.x;       // below 2^32 (checked on the host)
+    uint32_t am[4], av[4], sign[4], tm = 0, tv = 0;      // code + 8 base; 0: zero, ~0: not finite
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t c = 0, x = 0;
+        if (at + j < numel && at + j >= at) {
+            const uint32_t row = rows.of(at + j), col = at + j - row * e.width;
+            const long long from = index[row];
+            if (from >= 0 && from < src_rows) {
+                const long long i = from * e.width + col;
+                c = e.codes[i];
+                x = e.exps[i / QBLOCK];
+            }
+        }
+        const uint32_t mag = c & 0x7Fu, vc = c >> 8;
+        sign[j] = c & 0x80u;
+        am[j] = mag == 0u ? 0u : mag == 127u ? ~0u : mag + 8u * (x & 0xFFu);
+        av[j] = vc == 0u ? 0u : vc == 255u ? ~0u : vc + 8u * (x >> 8);
+        tm = max(tm, am[j] == ~0u ? 0u : am[j]);
+        tv = max(tv, av[j] == ~0u ? 0u : av[j]);
+    }
+    const int bm = max((int)(half_max(tm) >> 3) - 14, 1), bv = max((int)(half_max(tv) >> 3) - 30, 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int mc = am[j] == ~0u ? 127 : am[j] == 0u ? 0 : max((int)am[j] - 8 * bm, 0), vc = av[j] == ~0u ? 255 : av[j] == 0u ? 0 : max((int)av[j] - 8 * bv, 1);
+        if (at + j < numel && at + j >= at) e.out_codes[at + j] = (uint16_t)(vc << 8 | sign[j] | mc);
+    }
+    if ((threadIdx.x & 31) == 0 && at < numel) e.out_exps[at / QBLOCK] = (uint16_t)(bm | bv << 8);
+}
+
 // ------------------------------------------------------------------------------------------------ global norm
 // Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split, and the squares of large
 // or small f32 gradients would leave its range.  The sums are split over the workgroups by position alone and joined in a fixed order.
@@ -650,6 +691,9 @@ bool disjoint(std::vector<Range>& r) {
     return true;
 }
 
+// the multiplier of Rows::of for a width above 1
+uint32_t row_magic(uint32_t w) { return (uint32_t)(((1ull << 32) * ((2ull << (31 - __builtin_clz(w - 1))) - w)) / w + 1); }
+
 uint32_t tiles_of(long long numel) { return (uint32_t)((numel + TILE_ELEMS - 1) / TILE_ELEMS); }
 
 struct StepCall {
@@ -673,7 +717,7 @@ int launch_step(const StepCall& c, int k, StepHyper& h, double inv_bc1, const gs
             e.wd = c.wd[k];
             const uint32_t w = dev->row_width && dev->row_width[k] > 0 ? (uint32_t)dev->row_width[k] : 0u;
             t.row_width[n] = w;
-            if (w > 1) t.row_magic[n] = (uint32_t)(((1ull << 32) * ((2ull << (31 - __builtin_clz(w - 1))) - w)) / w + 1);
+            if (w > 1) t.row_magic[n] = row_magic(w);
             if (dev->row_freeze && dev->group_frozen[k] && t.row_width[n] > 0) e.word |= 1ull << 38;
         } else {
             e.scale[0] = (float)(c.lr[k] * inv_bc1);
@@ -707,7 +751,7 @@ int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, ui
             return fail("gsicp_adamw_step: the device form needs learning rates, a step counter and bump_step 0, 1 or 2");
         if ((dev->live_rows || dev->row_freeze || dev->grad_rows) && !dev->row_width) return fail("gsicp_adamw_step: live rows and row masks need row_width");
         if (dev->row_freeze && !dev->group_frozen) return fail("gsicp_adamw_step: row_freeze needs group_frozen");
-        if (Q8 && (dev->live_rows || dev->row_freeze)) return fail("gsicp_adamw_step_8bit: live rows and frozen rows would share block exponents with rows that move");
+        if (Q8 && dev->row_freeze) return fail("gsicp_adamw_step_8bit: frozen rows would share block exponents with rows that move");
     } else if (step < 1 || (c.n > 0 && !c.lr)) {
         return fail("gsicp_adamw_step: the host form needs learning rates and a step count of at least 1");
     }
@@ -819,6 +863,49 @@ int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* co
         else hipLaunchKernelGGL((adamw_decode_kernel<BF16, false>), grid, dim3(256), 0, stream, t);
     }
     if (hipGetLastError() != hipSuccess) { g_last_error = "gsicp_adamw_decode: kernel launch failed"; return -1; }
+    return 0;
+}
+
+int gsicp_adamw_gather_rows(int n, const uint16_t* const* moments, const uint16_t* const* block_exps, uint16_t* const* out_moments, uint16_t* const* out_exps,
+                            const long long* row_width, const long long* index, long long n_rows, long long src_rows, void* stream_v) {
+    hipStream_t stream = (hipStream_t)stream_v;
+    if (n < 0 || n_rows < 0 || src_rows < 0 || (n > 0 && (!moments || !block_exps || !out_moments || !out_exps || !row_width))) return fail("gsicp_adamw_gather_rows: missing arrays");
+    if (n > 0 && n_rows > 0 && !index) return fail("gsicp_adamw_gather_rows: missing index");
+    try {
+        std::vector<Range> ranges;
+        for (int k = 0; k < n; ++k) {
+            const long long w = row_width[k];
+            if (w <= 0 || n_rows == 0 || src_rows == 0 || n_rows > 0xFFFFFFFFll / w || src_rows > MAX_NUMEL / w) continue;       // empty, or refused below
+            auto add = [&](const void* q, long long numel, bool written) { ranges.push_back({(uintptr_t)q, (uintptr_t)q + 2 * (size_t)numel, written}); };
+            add(moments[k], src_rows * w, false); add(block_exps[k], (src_rows * w + QBLOCK - 1) / QBLOCK, false);
+            add(out_moments[k], n_rows * w, true); add(out_exps[k], (n_rows * w + QBLOCK - 1) / QBLOCK, true);
+        }
+        if (!disjoint(ranges)) return fail("gsicp_adamw_gather_rows: the result overlaps its source or itself");
+    } catch (const std::exception& ex) { g_last_error = ex.what(); return -1; }
+    for (int k = 0; k < n; ++k) {
+        const long long w = row_width[k];
+        if (w < 0 || (w > 0 && (n_rows > 0xFFFFFFFFll / w || src_rows > MAX_NUMEL / w))) return fail("gsicp_adamw_gather_rows: a tensor has less than 2^32 elements");
+        if (w == 0 || n_rows == 0) continue;
+        if (!moments[k] || !block_exps[k] || !out_moments[k] || !out_exps[k]) return fail("gsicp_adamw_gather_rows: null pointer of a tensor that is not empty");
+    }
+    for (int k = 0; k < n;) {
+        GatherTable t = {};
+        int m = 0;
+        unsigned long long tiles = 0;
+        for (; k < n && m < TABLE; ++k) {
+            const long long numel = n_rows * row_width[k];
+            if (numel == 0) continue;
+            if (tiles + tiles_of(numel) > STEP_TILES) break;
+            const uint32_t w = (uint32_t)row_width[k];
+            t.e[m] = {moments[k], block_exps[k], out_moments[k], out_exps[k], w, w > 1 ? row_magic(w) : 0u};
+            t.first[m++] = (uint32_t)tiles;
+            tiles += tiles_of(numel);
+        }
+        for (int i = m; i < 64; ++i) t.first[i] = LAST;
+        if (m == 0) break;
+        hipLaunchKernelGGL(adamw_gather_kernel, dim3((unsigned)tiles), dim3(64), 0, stream, t, index, (uint32_t)n_rows, src_rows);
+    }
+    if (hipGetLastError() != hipSuccess) { g_last_error = "gsicp_adamw_gather_rows: kernel launch failed"; return -1; }
     return 0;
 }
 

@@ -21,13 +21,18 @@ full-capacity buffers (never re-created), the optimiser's moments are the full-c
 device int (`live_count`).  `append` writes rows in place and bumps the count; `prune` compacts into the second buffer set and copies the
 survivors back.  Kernels that take `live_count` (rasteriser, activations, FusedAdam — include/gsicp_hip.h `live_rows_dev`) ignore the
 rows behind it, so a captured mapper iteration (gs_icp_slam_amd/graph.py) survives keyframes and pruning without being re-captured.
+
+`GaussianStore(moment_bits=8)` keeps the moments of FusedAdamW(state_bits=8) instead (2 bytes per element for both, and 2 per 128): pruning re-blocks them
+(optim.gather_moments_8bit); rows behind the live ones hold zero codes.
 """
 import ctypes
+import math
 
 import torch
 import torch.nn as nn
 
 from . import _lib
+from .optim import gather_moments_8bit
 
 PARAM_NAMES = ("xyz", "f_dc", "f_rest", "opacity", "scaling", "rotation")
 
@@ -54,9 +59,11 @@ def rows_from_gicp(points, colors, rots, scales, z_values, trackable_idxs=None, 
 
 
 class GaussianStore:
-    def __init__(self, capacity, n_rest=0, device="cuda", stable=False):
+    def __init__(self, capacity, n_rest=0, device="cuda", stable=False, moment_bits=32):
+        if moment_bits not in (8, 32):
+            raise ValueError("GaussianStore: moment_bits is 32 or 8")
         self.capacity, self.n_rest, self.device = int(capacity), int(n_rest), torch.device(device)
-        self.stable = bool(stable)
+        self.stable, self.moment_bits = bool(stable), moment_bits
         self.n = 0
         shapes = {"xyz": (3,), "f_dc": (1, 3), "f_rest": (self.n_rest, 3), "opacity": (1,), "scaling": (3,), "rotation": (4,)}
         self._shapes = shapes
@@ -65,8 +72,11 @@ class GaussianStore:
         def new_set():
             s = {}
             for k, sh in shapes.items():
-                for role in ("p", "m", "v"):                       # parameter, exp_avg, exp_avg_sq
+                for role in ("p", "m", "v") if moment_bits == 32 else ("p",):      # parameter, exp_avg, exp_avg_sq
                     s[(role, k)] = torch.zeros((self.capacity,) + sh, **f32)
+                if moment_bits == 8:                               # codes of both moments, exponents of their blocks
+                    s[("c", k)] = torch.zeros((self.capacity,) + sh, dtype=torch.int16, device=self.device)
+                    s[("x", k)] = torch.zeros(self._blocks(k, self.capacity), dtype=torch.int16, device=self.device)
             s[("aux", "xyz_gradient_accum")] = torch.zeros((self.capacity, 1), **f32)
             s[("aux", "denom")] = torch.zeros((self.capacity, 1), **f32)
             s[("aux", "max_radii2D")] = torch.zeros((self.capacity,), **f32)
@@ -84,8 +94,22 @@ class GaussianStore:
     def _buf(self, role, name):
         return self._sets[self._cur][(role, name)]
 
+    def _blocks(self, name, rows):
+        """128-element blocks of `rows` rows of a parameter's 8-bit moments."""
+        return (rows * math.prod(self._shapes[name]) + 127) // 128
+
+    def _len(self, role, name):
+        return self._blocks(name, self.n) if role == "x" else self.n
+
     def view(self, role, name):
-        return self._buf(role, name)[: self.n]
+        return self._buf(role, name)[: self._len(role, name)]
+
+    def _state_views(self, name, full):
+        """The optimiser state entries of a parameter: views of the live part, or the full-capacity buffers of set 0 (stable mode)."""
+        get = (lambda role: self._sets[0][(role, name)]) if full else (lambda role: self.view(role, name))
+        if self.moment_bits == 8:
+            return {"moments": get("c"), "block_exps": get("x")}
+        return {"exp_avg": get("m"), "exp_avg_sq": get("v")}
 
     @property
     def trackable_mask(self):
@@ -118,8 +142,7 @@ class GaussianStore:
             new_p = self.params[name]
             group["params"][0] = new_p
             if st is not None:
-                st["exp_avg"] = self.view("m", name)
-                st["exp_avg_sq"] = self.view("v", name)
+                st.update(self._state_views(name, full=False))
                 self.optimizer.state[new_p] = st
         del old
 
@@ -131,9 +154,9 @@ class GaussianStore:
         groups = [{"params": [self.params[k]], "lr": float(lrs[k]), "name": k} for k in PARAM_NAMES]
         self.optimizer = optimizer_cls(groups, **kw)
         # the moments live in the store from the first step on (a lazily created zeros_like() would sit outside it)
-        if getattr(self.optimizer, "state_bits", 32) != 32:
+        if getattr(self.optimizer, "state_bits", 32) != self.moment_bits:
             self.optimizer = None
-            raise RuntimeError("GaussianStore.attach: the store's moments are 32-bit (rows of 8-bit ones cannot move between blocks that share an exponent)")
+            raise RuntimeError(f"GaussianStore.attach: the store keeps {self.moment_bits}-bit moments, the optimiser another width")
         fused = hasattr(self.optimizer, "capturable") and type(self.optimizer).__name__ in ("FusedAdam", "FusedAdamW")
         shared_step = torch.zeros((), dtype=torch.int32, device=self.device) if (fused and self.optimizer.capturable) else None
         for k in PARAM_NAMES:
@@ -141,8 +164,7 @@ class GaussianStore:
                 step = shared_step if shared_step is not None else 0
             else:
                 step = torch.tensor(0.0)                           # torch.optim.Adam keeps a float32 CPU scalar
-            m, v = (self._sets[0][("m", k)], self._sets[0][("v", k)]) if self.stable else (self.view("m", k), self.view("v", k))
-            self.optimizer.state[self.params[k]] = {"step": step, "exp_avg": m, "exp_avg_sq": v}
+            self.optimizer.state[self.params[k]] = {"step": step, **self._state_views(k, full=self.stable)}
         if self.stable and hasattr(self.optimizer, "set_live_rows"):
             self.optimizer.set_live_rows(self._n_dev)
         return self.optimizer
@@ -159,8 +181,8 @@ class GaussianStore:
         with torch.no_grad():
             for name in PARAM_NAMES:
                 self._buf("p", name)[lo:hi].copy_(new[name].reshape((k,) + self._shapes[name]))
-                self._buf("m", name)[lo:hi].zero_()
-                self._buf("v", name)[lo:hi].zero_()
+                for role in ("m", "v") if self.moment_bits == 32 else ("c",):
+                    self._buf(role, name)[lo:hi].zero_()
             for aux in ("xyz_gradient_accum", "denom", "max_radii2D"):
                 self._buf("aux", aux)[:hi].zero_()
             tm = self._buf("aux", "trackable_mask")[lo:hi]
@@ -192,21 +214,22 @@ class GaussianStore:
         for _ in range(2):
             s = {}
             for key, t in old_sets[0].items():
-                s[key] = torch.zeros((new_capacity,) + tuple(t.shape[1:]), dtype=t.dtype, device=self.device)
+                rows = self._blocks(key[1], new_capacity) if key[0] == "x" else new_capacity
+                s[key] = torch.zeros((rows,) + tuple(t.shape[1:]), dtype=t.dtype, device=self.device)
             new_sets.append(s)
         with torch.no_grad():
             src = old_sets[old_cur]
             for key, t in src.items():
-                if n > 0 and t[0].numel() > 0:
-                    new_sets[0][key][:n].copy_(t[:n])
+                if n > 0 and t.numel() > 0:
+                    rows = self._len(*key)
+                    new_sets[0][key][:rows].copy_(t[:rows])
         self._sets, self._cur = new_sets, 0
         if self.params:
             if self.stable:
                 for k in PARAM_NAMES:
                     self.params[k].data = self._sets[0][("p", k)]
                     if self.optimizer is not None and self.params[k] in self.optimizer.state:
-                        st = self.optimizer.state[self.params[k]]
-                        st["exp_avg"], st["exp_avg_sq"] = self._sets[0][("m", k)], self._sets[0][("v", k)]
+                        self.optimizer.state[self.params[k]].update(self._state_views(k, full=True))
             else:
                 self._rebind()
         del old_sets, f32
@@ -223,7 +246,7 @@ class GaussianStore:
         n_old = self.n
         keep = (~remove_mask.reshape(-1)[: self.n].to(device=self.device, dtype=torch.bool)).contiguous().view(torch.uint8)
         src, dst = self._sets[self._cur], self._sets[self._cur ^ 1]
-        keys = list(src.keys())
+        keys = [key for key in src if key[0] not in ("c", "x")]
         n_arr = len(keys)
         S = (ctypes.c_void_p * n_arr)(*[src[k].data_ptr() for k in keys])
         D = (ctypes.c_void_p * n_arr)(*[dst[k].data_ptr() for k in keys])
@@ -242,23 +265,27 @@ class GaussianStore:
                                                ctypes.c_void_p(self._scratch.data_ptr()), ctypes.c_void_p(self._n_dev.data_ptr()), stream),
                        "gsicp_store_compact")
         self.n = int(self._n_dev.item())
+        if self.moment_bits == 8:      # their rows come into other blocks: re-blocked, not copied
+            of = lambda s, role, rows: [s[(role, name)][:rows(name)] for name in PARAM_NAMES]   # noqa: E731
+            gather_moments_8bit(of(src, "c", lambda name: n_old), of(src, "x", lambda name: self._blocks(name, n_old)), torch.nonzero(keep).reshape(-1),
+                                out=(of(dst, "c", lambda name: self.n), of(dst, "x", lambda name: self._blocks(name, self.n))))
+            keys = keys + [(role, name) for name in PARAM_NAMES for role in ("c", "x")]
         if self.stable:
             # addresses must not move: the survivors go back into set 0 (the compaction cannot run in place: a parallel scatter would
             # overwrite rows other threads have not read yet).  Rows behind the new count keep stale values; nothing reads them, and append()
             # rewrites parameters and zeroes moments of the rows it claims.
             with torch.no_grad():
                 for k in keys:
-                    if src[k][0].numel() > 0 and self.n > 0:
-                        src[k][: self.n].copy_(dst[k][: self.n])
+                    if src[k].numel() > 0 and self.n > 0:
+                        src[k][: self._len(*k)].copy_(dst[k][: self._len(*k)])
                 # the freed tail [n_new, n_old) still holds copies of old Gaussians; a consumer that ignores `live_count` (torch.optim.Adam,
                 # a custom rasteriser factory, a checkpoint written from `params` instead of `live()`) would render / update them.  Make them
                 # inert: opacity far below every threshold (sigmoid(-30) = 1e-13 < 1/255: culled by the rasteriser), moments zero.
                 if n_old > self.n:
                     src[("p", "opacity")][self.n:n_old].fill_(-30.0)
                     for name in PARAM_NAMES:
-                        if src[("m", name)][0].numel() > 0:
-                            src[("m", name)][self.n:n_old].zero_()
-                            src[("v", name)][self.n:n_old].zero_()
+                        for role in ("m", "v") if self.moment_bits == 32 else ("c",):
+                            src[(role, name)][self.n:n_old].zero_()
             return self.params
         self._cur ^= 1
         self._rebind()

@@ -21,6 +21,7 @@ and `FusedAdamW`, the optimiser over them.  `max_norm=` clips by the global norm
 """
 import array
 import ctypes
+import math
 
 import torch
 
@@ -396,12 +397,46 @@ def decode_moments(moments, block_exps, dtype=torch.float32):
     return exp_avgs, exp_avg_sqs
 
 
+def gather_moments_8bit(moments, block_exps, index, out=None):
+    """Rows of 8-bit moments, as `t[index]` would take them from their values: -> (moments, block_exps), lists of new tensors (or `out`, two lists of contiguous int16 tensors that
+    hold at least that much; nothing behind it is written).  All tensors have the same number of rows; index: int64 on their device, rows outside come out zero.  Values are moved
+    exactly, except those that fall below the smallest code of the 128-element block they come into (first moments become zero, second that code)."""
+    moments, block_exps = list(moments), list(block_exps)
+    if not moments:
+        return [], []
+    what = "gather_moments_8bit"
+    device, current, stream, n, at, keep = _pack(what, ("moments", "block_exps"), "cb", moments, block_exps)
+    dev = moments[0].device
+    rows = moments[0].shape[0] if moments[0].dim() else -1
+    if any(t.dim() == 0 or t.shape[0] != rows for t in moments):
+        raise RuntimeError(f"{what}: every tensor must have the same number of rows")
+    if index.dtype != torch.int64 or index.device != dev or index.dim() != 1 or not index.is_contiguous():
+        raise RuntimeError(f"{what}: index must be a contiguous one-dimensional int64 tensor on the device of the moments")
+    count = index.numel()
+    widths = array.array("q", [math.prod(t.shape[1:]) for t in moments])
+    if out is None:
+        out = ([torch.empty((count,) + tuple(t.shape[1:]), dtype=torch.int16, device=dev) for t in moments],
+               [torch.empty((count * w + _BLOCK - 1) // _BLOCK, dtype=torch.int16, device=dev) for w in widths])
+    else:
+        for ts, need in ((out[0], [count * w for w in widths]), (out[1], [(count * w + _BLOCK - 1) // _BLOCK for w in widths])):
+            if len(ts) != n or any(t.dtype != torch.int16 or t.device != dev or not t.is_contiguous() or t.numel() < k for t, k in zip(ts, need)):
+                raise RuntimeError(f"{what}: out must be contiguous int16 tensors on the device of the moments, large enough")
+    if rows == 0:
+        for ts, need in zip(out, ([count * w for w in widths], [(count * w + _BLOCK - 1) // _BLOCK for w in widths])):
+            for t, k in zip(ts, need):
+                t.view(-1)[:k].zero_()
+        return out
+    o_c, o_x = (array.array("Q", [t.data_ptr() for t in ts]) for ts in out)
+    _call("gsicp_adamw_gather_rows", device, current, n, at, at + 8 * n, _at(o_c), _at(o_x), _at(widths), index.data_ptr(), count, rows, stream)
+    return out
+
+
 class FusedAdamW(FusedAdam):
     """torch.optim.AdamW (amsgrad and maximize off) over any number of f32, bf16 and f16 parameters, one launch per 64 of them with the same betas, eps and step count.
 
     state_bits      32: state[p] = {"step", "exp_avg", "exp_avg_sq"} (f32; torch's layout, so GaussianStore and the reference's append / prune keep working)
-                    8: state[p] = {"step", "moments", "block_exps"} — adamw_step_8bit's; `moments(p)` gives their values.  A map that grows or is pruned needs 32: its rows
-                    would move between blocks that share an exponent (GaussianStore.attach refuses)
+                    8: state[p] = {"step", "moments", "block_exps"} — adamw_step_8bit's; `moments(p)` gives their values.  For a map that grows or is pruned:
+                    GaussianStore(moment_bits=8)
     master_weights  16-bit parameters keep an f32 copy in state[p]["master"] that takes the update
     max_grad_norm   clip by the global norm of all gradients of the step; `last_grad_norm` is then a 0-dim device tensor
     seed            of the stochastic rounding of 8-bit moments
@@ -423,8 +458,7 @@ class FusedAdamW(FusedAdam):
         self.last_grad_norm = None
 
     def set_live_rows(self, n_dev):
-        if n_dev is not None and self.state_bits == 8:
-            raise RuntimeError("FusedAdamW(state_bits=8): a capacity-backed map needs 32-bit moments (rows behind the live count would share block exponents with rows that move)")
+        """As in FusedAdam; with 8-bit moments the codes of the rows behind the live ones must be zero (as GaussianStore keeps them): they share the last live block's exponents."""
         super().set_live_rows(n_dev)
 
     def set_row_freeze(self, mask, group_names):

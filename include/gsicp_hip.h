@@ -437,13 +437,18 @@ int gsicp_adamw_step(int n, void* const* params, const void* const* grads, float
  * 2^((c >> 3) + b - 127), 0 is zero (whatever its sign bit); code 127 of the first moment is NaN, 255 of the second infinity.  All-zero arrays are the state before the first step.  Moments are
  * rounded stochastically: with mix(x) = { x ^= x >> 16; x *= 0x7FEB352D; x ^= x >> 15; x *= 0x846CA68B; x ^= x >> 16 } and L = the eight odd words of lane_word (adamw.hip),
  * element j of the tensor at place[k] (HOST int[n]; NULL: k) takes the halves of mix((j >> 3) ^ mix(seed + step * 0x9E3779B1 + place * 0x85EBCA6B)) * L[j & 7]: the same
- * seed, step and place give the same bits.  The device form takes no live_rows and no row_freeze. */
+ * seed, step and place give the same bits.  The device form takes no row_freeze; with live_rows, the rows behind them hold zero codes (they share the last live block's
+ * exponents). */
 int gsicp_adamw_step_8bit(int n, void* const* params, const void* const* grads, float* const* masters, uint16_t* const* moments, uint16_t* const* block_exps,
                           const long long* numel, const int* dtype, const double* lr, const double* weight_decay, double beta1, double beta2, double eps, int step,
                           uint32_t seed, const int* place, const float* clip, const gsicp_adamw_device* dev, void* stream);
 /* Values of 8-bit moments, as f32 (dtype 0) or bf16 (1; exact). */
 int gsicp_adamw_decode(int n, const uint16_t* const* moments, const uint16_t* const* block_exps, void* const* exp_avg, void* const* exp_avg_sq, const long long* numel,
                        int dtype, void* stream);
+/* Rows of 8-bit moments (pruning, reordering): row r of out is row index[r] (DEVICE int64[n_rows]) of the source, for n tensors of src_rows rows of row_width[k] (HOST) elements
+ * at once; rows outside [0, src_rows) come out zero.  Values are moved exactly, except those that fall below the smallest code of their new block.  Out of place. */
+int gsicp_adamw_gather_rows(int n, const uint16_t* const* moments, const uint16_t* const* block_exps, uint16_t* const* out_moments, uint16_t* const* out_exps,
+                            const long long* row_width, const long long* index, long long n_rows, long long src_rows, void* stream);
 /* *norm_out = 2-norm over all elements of n tensors (dtype[k] as above; squares and sums in double, fixed order), *clip_out (may be NULL) = min(1, max_norm /
  * (norm + 1e-6)) — the factor of torch.nn.utils.clip_grad_norm_ —, or 1 when max_norm <= 0.  norm_out, clip_out: DEVICE; scratch: DEVICE, 8-byte aligned,
  * gsicp_grad_norm_scratch_bytes() bytes (0 for few small tensors: scratch may then be NULL), needs no initialisation and holds nothing afterwards. */

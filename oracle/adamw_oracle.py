@@ -62,6 +62,25 @@ def encode(m, v, um, uv):
     return (mc | vc << 8).reshape(-1)[:n].astype(np.uint16), (bm | bv << 8).reshape(-1).astype(np.uint16)
 
 
+def gather(moments, exps, width, index, rows):
+    """Rows of 8-bit moments by index (outside: zero), re-blocked: each value keeps itself unless it is below the smallest code of its new block."""
+    c = np.asarray(moments).view(np.uint16).astype(np.int64).reshape(rows, width)
+    e = np.repeat(np.asarray(exps).view(np.uint16).astype(np.int64), BLOCK)[:c.size].reshape(rows, width)
+    inside = (index >= 0) & (index < rows)
+    take = lambda x: np.where(inside[:, None], x[np.where(inside, index, 0)], 0).reshape(-1)       # noqa: E731
+    c, e = take(c), take(e)
+    mag, sign, vc = c & 127, c & 128, c >> 8
+    out = []
+    for code, base, top, below in ((mag, e & 255, 127, 14), (vc, e >> 8, 255, 30)):
+        special = code == top
+        absolute = np.where((code > 0) & ~special, code + 8 * base, 0)
+        new = np.maximum((blocks_of(absolute).max(1) >> 3) - below, 1)
+        moved = np.maximum(absolute - 8 * np.repeat(new, BLOCK)[:absolute.size], 0 if top == 127 else 1)
+        out.append((np.where(special, top, np.where(absolute > 0, moved, 0)), new))
+    (m, bm), (v, bv) = out
+    return (m | sign | v << 8).astype(np.uint16), (bm | bv << 8).astype(np.uint16)
+
+
 def step32(m, v, g, betas, clip=None):
     """The moments of one step in float32, each operation rounded by itself."""
     f = np.float32

@@ -75,6 +75,27 @@ def test_ends_of_the_range():
     assert exps[0] == (1 | 1 << 8) and (codes == 1 << 8).all()
 
 
+def test_gathered_rows_keep_their_values():
+    rng = np.random.default_rng(0)
+    rows, width = 500, 5
+    m = (rng.normal(size=rows * width) * np.exp(3 * rng.normal(size=rows * width))).astype(np.float32)
+    v = (rng.normal(size=rows * width) ** 2 * np.exp(6 * rng.normal(size=rows * width))).astype(np.float32)
+    m[::7], v[::11], m[3], v[4] = 0, 0, np.nan, np.inf
+    codes, exps = ao.encode(m, v, *ao.random_bits(rows * width, 1, 1, 0))
+    a, b = ao.decode(codes, exps)
+    index = np.concatenate([np.flatnonzero(rng.random(rows) < 0.6), [3, 3, -1, rows, 0]])
+    c2, e2 = ao.gather(codes, exps, width, index, rows)
+    a2, b2 = ao.decode(c2, e2)
+    inside = (index >= 0) & (index < rows)
+    want = [np.where(inside[:, None], x.reshape(rows, width)[np.where(inside, index, 0)], 0.0).reshape(-1) for x in (a, b)]
+    low = lambda shift: np.repeat(1.125 * 2.0 ** ((e2.astype(int) >> shift & 255) - 127), 128)[:c2.size]      # noqa: E731
+    for got, w, lo, floor in ((a2, want[0], low(0), 0.0), (b2, want[1], low(8), None)):
+        small = (np.abs(w) < lo) & (w != 0)
+        np.testing.assert_array_equal(got[~small], w[~small])
+        np.testing.assert_array_equal(got[small], lo[small] if floor is None else 0.0)
+    assert np.array_equal(ao.gather(*ao.gather(codes, exps, width, np.arange(rows), rows), width, np.arange(rows), rows)[0], ao.gather(codes, exps, width, np.arange(rows), rows)[0])
+
+
 def _arrays(n, **kw):
     d = dict(params=[4096 * (k + 1) for k in range(n)], grads=[1 << 20] * n, masters=None, s0=[(1 << 21) + 4096 * k for k in range(n)], s1=[(1 << 22) + 4096 * k for k in range(n)],
              numel=[100] * n, dtype=[0] * n, lr=[1e-3] * n, wd=[0.0] * n)
@@ -114,7 +135,7 @@ def test_c_abi_refuses_before_it_launches():
             assert step(eight=eight, dev=ctypes.addressof(d)) == -2
         d = D(lr_dev=64, step_dev=64, grad_rows=64, row_width=ctypes.addressof(width))
         assert step(eight=eight, dev=ctypes.addressof(d), dtype=[0, 1]) == -2 and step(eight=eight, dev=ctypes.addressof(d), numel=[100, 1 << 32]) == -2
-    d = D(lr_dev=64, step_dev=64, live_rows=64, row_width=ctypes.addressof(width))
+    d = D(lr_dev=64, step_dev=64, row_freeze=64, group_frozen=ctypes.addressof(width), row_width=ctypes.addressof(width))
     assert step(eight=True, dev=ctypes.addressof(d)) == -2
     assert b"gsicp_adamw_step_8bit" in lib.gsicp_last_error()
     assert lib.gsicp_adamw_step(-1, *[None] * 9, 0.9, 0.999, 1e-8, 1, None, None, None) == -2 and lib.gsicp_adamw_decode(-1, *[None] * 5, 0, None) == -2
@@ -123,6 +144,11 @@ def test_c_abi_refuses_before_it_launches():
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(0), k(5), 0, None) == -2
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(64), k(5), 2, None) == -2
     assert lib.gsicp_adamw_decode(1, one(64), one(64), one(64), one(64), k(-5), 0, None) == -2
+    gather = lambda c, x, oc, ox, w, index, n, src: lib.gsicp_adamw_gather_rows(1, one(c), one(x), one(oc), one(ox), k(w), index, n, src, None)      # noqa: E731
+    assert gather(1 << 12, 1 << 20, 1 << 21, 1 << 22, 3, None, 5, 9) == -2 and gather(1 << 12, 1 << 20, 0, 1 << 22, 3, 64, 5, 9) == -2
+    assert gather(1 << 12, 1 << 20, 1 << 12, 1 << 22, 3, 64, 5, 9) == -2 and gather(1 << 12, 1 << 20, (1 << 12) + 52, 1 << 22, 3, 64, 5, 9) == -2       # in place, into the last row
+    assert gather(1 << 12, 1 << 20, 1 << 21, 1 << 22, 3, 64, (1 << 32) // 3 + 1, 9) == -2 and gather(1 << 12, 1 << 20, 1 << 21, 1 << 22, -1, 64, 5, 9) == -2
+    assert gather(1 << 12, 1 << 20, 1 << 21, 1 << 22, 3, 64, -5, 9) == -2 and gather(1 << 12, 1 << 20, 1 << 21, 1 << 22, 3, 64, 5, -9) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(0), 0.0, None, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(5), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(0), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
@@ -155,6 +181,14 @@ def test_python_layer_has_no_cpu_path_and_refuses_bad_options():
     with pytest.raises(RuntimeError):
         store.attach(FusedAdamW, lrs, state_bits=8)
     assert store.optimizer is None
+    with pytest.raises(ValueError):
+        GaussianStore(16, device="cpu", moment_bits=16)
+    small = GaussianStore(16, n_rest=2, device="cpu", moment_bits=8)
+    for cls, kw in ((FusedAdamW, {}), (torch.optim.Adam, {})):
+        with pytest.raises(RuntimeError):
+            small.attach(cls, lrs, **kw)
+    opt = small.attach(FusedAdamW, lrs, state_bits=8)
+    assert all(opt.state[q]["moments"].shape == q.shape and opt.state[q]["block_exps"].numel() == -(-q.numel() // 128) for q in small.params.values())
     opt = store.attach(FusedAdamW, lrs, weight_decay=0.1)
     assert all(opt.state[q]["step"] == 0 and opt.state[q]["exp_avg"].shape == q.shape for q in store.params.values())
     assert all(g["weight_decay"] == 0.1 for g in opt.param_groups)

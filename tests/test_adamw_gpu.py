@@ -258,6 +258,45 @@ def test_decode_keeps_shapes_over_many_tensors():
     assert decode_moments([], []) == ([], [])
 
 
+@pytest.mark.parametrize("rows,widths", [(1, [1]), (40, [3, 3, 0, 1, 3, 4]), (5000, [3, 45, 1, 4, 128, 2, 7]), (3, [1000, 129]), (90, [5, 1] * 40)])
+def test_gathered_rows_of_8_bit_moments(rows, widths):
+    from gs_icp_slam_amd.optim import gather_moments_8bit
+    rng = np.random.default_rng(rows)
+    src = []
+    for k, w in enumerate(widths):
+        n = rows * w
+        m, v = (rng.normal(size=n) * np.exp(3 * rng.normal(size=n))).astype(np.float32), (rng.normal(size=n) ** 2 * np.exp(6 * rng.normal(size=n))).astype(np.float32)
+        m[rng.random(n) < 0.1], v[rng.random(n) < 0.1] = 0, 0
+        m[rng.random(n) < 0.01], v[rng.random(n) < 0.01] = np.nan, np.inf
+        src.append(ao.encode(m, v, *ao.random_bits(n, 1, 1, k)))
+    c, x = ([torch.from_numpy(s[i].view(np.int16).copy()).cuda() for s in src] for i in (0, 1))
+    c = [t.view(rows, w) for t, w in zip(c, widths)]
+    for index in (np.flatnonzero(rng.random(rows) < 0.5), rng.integers(0, rows, 2 * rows), np.arange(rows)[::-1].copy(), np.array([-1, rows, 0, rows - 1, -(1 << 40), 1 << 40]),
+                  np.zeros(0, dtype=np.int64)):
+        at = torch.from_numpy(index.astype(np.int64)).cuda()
+        oc, ox = gather_moments_8bit(c, x, at)
+        big = ([torch.full((index.size * w + 9,), 7, dtype=torch.int16, device="cuda") for w in widths], [torch.full((-(-index.size * w // 128) + 3,), 7, dtype=torch.int16, device="cuda")
+                                                                                                     for w in widths])
+        gather_moments_8bit(c, x, at, out=big)
+        for k, w in enumerate(widths):
+            codes, exps = ao.gather(*src[k], w, index, rows) if w else (np.zeros(0, np.uint16), np.zeros(0, np.uint16))
+            assert oc[k].shape == (index.size, w)
+            assert np.array_equal(oc[k].cpu().numpy().view(np.uint16).reshape(-1), codes) and np.array_equal(ox[k].cpu().numpy().view(np.uint16), exps), (k, w)
+            assert torch.equal(big[0][k][: codes.size], oc[k].view(-1)) and bool((big[0][k][codes.size:] == 7).all())
+            assert torch.equal(big[1][k][: exps.size], ox[k]) and bool((big[1][k][exps.size:] == 7).all())
+    empty = gather_moments_8bit([t[:0] for t in c], [t[:0] for t in x], torch.zeros(4, dtype=torch.int64, device="cuda"))
+    assert all(t.shape == (4, w) and not bool(t.any()) for t, w in zip(empty[0], widths))
+    with pytest.raises(RuntimeError):
+        gather_moments_8bit(c, x, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError):
+        gather_moments_8bit(c, x, torch.zeros(4, dtype=torch.int64))
+    if rows > 1:
+        with pytest.raises(RuntimeError):
+            gather_moments_8bit(c, x, torch.arange(rows, device="cuda"), out=([t.view(-1) for t in c], [t.clone() for t in x]))
+        with pytest.raises(RuntimeError):
+            gather_moments_8bit(c, x, torch.arange(rows, device="cuda"), out=([t.new_empty(max(t.numel() - 1, 0)) for t in c], [t.clone() for t in x]))
+
+
 # ------------------------------------------------------------------------------------------------ global norm
 @pytest.mark.parametrize("sizes", [[1], [0], [0, 0, 3], MANY, [7, 12] * 100, [3_000_001, 5]])
 def test_grad_norm_over_mixed_types(sizes):
@@ -522,30 +561,51 @@ def _rows(k, n_rest, seed):
     return {"xyz": r(k, 3), "f_dc": r(k, 1, 3), "f_rest": r(k, n_rest, 3), "opacity": r(k, 1), "scaling": r(k, 3), "rotation": r(k, 4)}
 
 
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("stable", [False, True])
 @pytest.mark.parametrize("n_rest", [0, 15])
-def test_a_map_that_grows_and_is_pruned(stable, n_rest):
-    """GaussianStore with FusedAdamW against the same rows kept as plain tensors, concatenated and indexed by hand."""
+def test_a_map_that_grows_and_is_pruned(stable, n_rest, bits):
+    """GaussianStore with FusedAdamW against the same rows kept as plain tensors, concatenated and indexed by hand (8-bit moments by the oracle's re-blocking)."""
     from gs_icp_slam_amd.gaussian_store import GaussianStore
-    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step
-    store = GaussianStore(4000, n_rest=n_rest, stable=stable)
+    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step, adamw_step_8bit
+    store = GaussianStore(4000, n_rest=n_rest, stable=stable, moment_bits=bits)
     first = _rows(1500, n_rest, 0)
     store.append(first)
-    opt = store.attach(FusedAdamW, LRS, lr=0.0, eps=1e-15, weight_decay=0.02, capturable=stable)
+    opt = store.attach(FusedAdamW, LRS, lr=0.0, eps=1e-15, weight_decay=0.02, capturable=stable, state_bits=bits, seed=6)
     p = {k: first[k].clone() for k in NAMES}
-    m, v = ({k: torch.zeros_like(p[k]) for k in NAMES} for _ in range(2))
+    blocks = lambda t: -(-t.numel() // 128)       # noqa: E731
+    if bits == 32:
+        s0, s1 = ({k: torch.zeros_like(p[k]) for k in NAMES} for _ in range(2))
+    else:
+        s0 = {k: torch.zeros(p[k].shape, dtype=torch.int16, device="cuda") for k in NAMES}
+        s1 = {k: torch.zeros(blocks(p[k]), dtype=torch.int16, device="cuda") for k in NAMES}
     t = 0
-    for op in ("step", "step", "grow", "step", "prune", "step", "grow", "step"):
+    for op in ("step", "step", "grow", "step", "prune", "step", "enlarge", "grow", "step", "prune", "prune", "step"):
         if op == "grow":
             new = _rows(700, n_rest, 100 + t)
             store.append(new)
             for k in NAMES:
                 p[k] = torch.cat((p[k], new[k]))
-                m[k], v[k] = (torch.cat((x[k], torch.zeros_like(new[k]))) for x in (m, v))
+                s0[k] = torch.cat((s0[k], torch.zeros(new[k].shape, dtype=s0[k].dtype, device="cuda")))
+                s1[k] = torch.cat((s1[k], torch.zeros_like(new[k]))) if bits == 32 else torch.cat((s1[k], s1[k].new_zeros(blocks(p[k]) - s1[k].numel())))
         elif op == "prune":
             remove = torch.rand(store.n, device="cuda") < 0.3
+            index = torch.nonzero(~remove).reshape(-1).cpu().numpy()
+            if bits == 8:
+                for k in NAMES:
+                    w = p[k][0].numel()
+                    if w:
+                        c, x = ao.gather(s0[k].cpu().numpy().reshape(-1), s1[k].cpu().numpy(), w, index, store.n)
+                        s0[k] = torch.from_numpy(c.view(np.int16)).cuda().view((len(index),) + p[k].shape[1:])
+                        s1[k] = torch.from_numpy(x.view(np.int16)).cuda()
+                    else:
+                        s0[k] = s0[k][~remove]
+            else:
+                s0, s1 = ({k: x[k][~remove].contiguous() for k in NAMES} for x in (s0, s1))
             store.prune(remove)
-            p, m, v = ({k: x[k][~remove].contiguous() for k in NAMES} for x in (p, m, v))
+            p = {k: p[k][~remove].contiguous() for k in NAMES}
+        elif op == "enlarge":
+            assert store.grow(6000)
         else:
             t += 1
             grads = {k: g * 0.1 for k, g in _rows(store.n, n_rest, 50 + t).items()}
@@ -554,17 +614,30 @@ def test_a_map_that_grows_and_is_pruned(stable, n_rest):
                 full[: store.n] = grads[k]
                 store.params[k].grad = full
             opt.step()
-            adamw_step([p[k] for k in NAMES], [grads[k] for k in NAMES], [m[k] for k in NAMES], [v[k] for k in NAMES], lr=[LRS[k] for k in NAMES], step=t, eps=1e-15,
-                       weight_decay=0.02)
+            kw = dict(lr=[LRS[k] for k in NAMES], step=t, eps=1e-15, weight_decay=0.02)
+            lists = [[x[k] for k in NAMES] for x in (p, grads, s0, s1)]
+            if bits == 32:
+                adamw_step(*lists, **kw)
+            else:
+                adamw_step_8bit(*lists, seed=6, **kw)
         assert store.n == p["xyz"].shape[0]
         for k in NAMES:
-            assert torch.equal(store.view("m", k), m[k]) and torch.equal(store.view("v", k), v[k]), (op, k)
-            if stable:        # the device form takes its bias corrections from another pow()
+            a, b = (store.view(r, k) for r in (("m", "v") if bits == 32 else ("c", "x")))
+            st = opt.state[store.params[k]]
+            for name, view in zip(("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps"), (a, b)):
+                assert st[name].data_ptr() == view.data_ptr() or view.numel() == 0, (op, k)
+            if bits == 32 or op == "step":
+                assert torch.equal(a, s0[k]) and torch.equal(b, s1[k]), (op, k)
+            else:                                    # blocks of new rows have no exponents yet, and zero codes
+                assert torch.equal(a, s0[k]), (op, k)
+            if stable:        # the device form takes its bias corrections in f32
                 assert p[k].numel() == 0 or (store.live(k) - p[k]).abs().max() <= t * 2.0 ** -22 * (5 + 10 * LRS[k]), (op, k)
             else:
                 assert torch.equal(store.live(k), p[k]), (op, k)
     if stable:
-        assert all(not bool(store.view("p", k).isnan().any()) and not bool(store.params[k].isnan().any()) for k in NAMES)
+        assert all(not bool(store.params[k].isnan().any()) for k in NAMES)
+        if bits == 8:
+            assert all(not bool(store._sets[0][("c", k)][store.n:].any()) for k in NAMES)
 
 
 @pytest.mark.parametrize("rows", [2777, 700_001])          # the larger one streams past the cache
@@ -726,8 +799,6 @@ def test_refusals_on_the_device():
     opt = FusedAdamW([torch.nn.Parameter(z(8))], state_bits=8, capturable=True)
     with pytest.raises(RuntimeError):
         opt.moments(opt.param_groups[0]["params"][0])
-    with pytest.raises(RuntimeError):
-        opt.set_live_rows(z(1, dt=torch.int32))
     with pytest.raises(RuntimeError):
         opt.set_row_freeze(z(8, dt=torch.int32), ("x",))
     p = torch.nn.Parameter(z(8, 2))

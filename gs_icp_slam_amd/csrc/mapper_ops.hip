@@ -868,6 +868,7 @@ __global__ void adam_bump_step_kernel(int* step_dev, const unsigned* __restrict_
 __global__ __launch_bounds__(256) void activations_forward_kernel(int P, const float* __restrict__ o_raw, const float* __restrict__ s_raw,
                                                                   const float4* __restrict__ q_raw, float* __restrict__ o,
                                                                   float* __restrict__ s, float4* __restrict__ q, const int* __restrict__ live_rows) {
+#pragma clang fp contract(off)   // as in the preprocess kernels, which apply the same getters inside (raw_params): the two forms round alike
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= P || (live_rows && i >= *live_rows)) return;     // rows behind the live count are not Gaussians: outputs left alone
     o[i] = 1.f / (1.f + expf(-o_raw[i]));
@@ -883,6 +884,7 @@ __global__ __launch_bounds__(256) void activations_backward_kernel(int P, const 
                                                                    const float* __restrict__ g_s, const float4* __restrict__ g_q,
                                                                    float* __restrict__ d_o_raw, float* __restrict__ d_s_raw,
                                                                    float4* __restrict__ d_q_raw, const int* __restrict__ live_rows) {
+#pragma clang fp contract(off)
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= P) return;
     if (live_rows && i >= *live_rows) {                        // not a Gaussian: zero gradient (its activations were never computed)
@@ -905,7 +907,8 @@ __global__ __launch_bounds__(256) void activations_backward_kernel(int P, const 
                 const float inv = 1.f / nn;
                 const float yx = r.x * inv, yy = r.y * inv, yz = r.z * inv, yw = r.w * inv;
                 const float dot = yx * g.x + yy * g.y + yz * g.z + yw * g.w;
-                out = make_float4((g.x - yx * dot) * inv, (g.y - yy * dot) * inv, (g.z - yz * dot) * inv, (g.w - yw * dot) * inv);
+                out = make_float4(__builtin_fmaf(-yx, dot, g.x) * inv, __builtin_fmaf(-yy, dot, g.y) * inv, __builtin_fmaf(-yz, dot, g.z) * inv,
+                                  __builtin_fmaf(-yw, dot, g.w) * inv);
             } else {
                 out = make_float4(g.x * 1e12f, g.y * 1e12f, g.z * 1e12f, g.w * 1e12f);
             }

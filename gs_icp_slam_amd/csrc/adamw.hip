@@ -276,7 +276,8 @@ __device__ __forceinline__ void adamw4(float p[4], float m[4], float v[4], const
         p[j] = __builtin_fmaf(-f.step_size, m[j] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[j], f.ibc2, f.eps)), p[j] * f.decay);
 }
 
-// New moments -> codes.  SPECIAL: some value of the wave is not finite.  top_m, top_v: bits of the largest value of the lane's block.
+constexpr uint32_t TOP_CODE = 0x7F700000u;      // 1.875 * 2^127: the last finite code of any base
+// New moments -> codes.  SPECIAL: some value of the wave is not finite, or so large that it could round up to what is not.
 template <bool SPECIAL>
 __device__ __forceinline__ void encode4(const float m[4], const float v[4], uint32_t bm, uint32_t bv, uint32_t word, uint32_t o[2]) {
     const float low = __uint_as_float((bm << 23) + (1u << 20)), low16 = low * 0x1p-16f, low17 = low16 * 0.5f;
@@ -284,7 +285,9 @@ __device__ __forceinline__ void encode4(const float m[4], const float v[4], uint
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const uint32_t r = word * ((threadIdx.x & 1) ? lane_word(j + 4) : lane_word(j));
-        const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = SPECIAL ? __float_as_uint(v[j]) & 0x7FFFFFFFu : __float_as_uint(v[j]);
+        uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = SPECIAL ? __float_as_uint(v[j]) & 0x7FFFFFFFu : __float_as_uint(v[j]);
+        const bool m_out = SPECIAL && mb >= 0x7F800000u, v_out = SPECIAL && vb >= 0x7F800000u;
+        if (SPECIAL) { mb = min(mb, TOP_CODE); vb = min(vb, TOP_CODE); }
         const float a = __uint_as_float(mb);
         uint32_t mc = ((mb + ((r << 4 & 0xFFFF0u) | 8u)) >> 20) - (bm << 3);
         // fma: low16 * (u + 1/2), rounded once
@@ -292,10 +295,8 @@ __device__ __forceinline__ void encode4(const float m[4], const float v[4], uint
         mc = (__float_as_uint(m[j]) >> 24 & 0x80u) | mc;
         const int vs = (int)((vb + ((r >> 12 & 0xFFFF0u) | 8u)) >> 20) - (int)(bv << 3);
         uint32_t vc = vb == 0u ? 0u : (uint32_t)max(vs, 1);
-        if (SPECIAL) {
-            if (mb >= 0x7F800000u) mc = 127u;
-            if (vb >= 0x7F800000u) vc = 255u;
-        }
+        if (m_out) mc = 127u;
+        if (v_out) vc = 255u;
         h[j] = vc << 8 | mc;
     }
     o[0] = h[1] << 16 | h[0];
@@ -403,7 +404,7 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
         }
     const uint32_t word = mix32(((uint32_t)tile * (TILE_ELEMS / 8) + (threadIdx.x >> 1)) ^ key);
     uint32_t bm, bv, o[2];
-    if (__ballot(max(tm, tv) >= 0x7F800000u) == 0) {
+    if (__ballot(max(tm, tv) > TOP_CODE) == 0) {
         bm = base_exponent(half_max(tm), 14);
         bv = base_exponent(half_max(tv), 30);
         encode4<false>(m, v, bm, bv, word, o);

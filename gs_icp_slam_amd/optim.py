@@ -280,7 +280,10 @@ def _at(a):
 def _doubles(what, name, value, n):
     if isinstance(value, (int, float)):
         return array.array("d", (value,)) * n
-    a = array.array("d", value)
+    try:
+        a = array.array("d", value)
+    except TypeError:                       # a scalar of another library
+        return array.array("d", (float(value),)) * n
     if len(a) != n:
         raise RuntimeError(f"{what}: {name} is a number or one per tensor ({len(a)} for {n} tensors)")
     return a

@@ -434,7 +434,8 @@ int gsicp_adamw_step(int n, void* const* params, const void* const* grads, float
                      const float* clip, const gsicp_adamw_device* dev, void* stream);
 /* The same step with both moments in 8 bits: moments (uint16[numel]: low byte sign and 7-bit code of exp_avg, high byte code of exp_avg_sq) and block_exps
  * (uint16[ceil(numel / 128)]: low / high byte the base exponent of the block's first / second moments).  A code c > 0 with base b is (1 + (c & 7) / 8) *
- * 2^((c >> 3) + b - 127), 0 is zero (whatever its sign bit); code 127 of the first moment is NaN, 255 of the second infinity.  All-zero arrays are the state before the first step.  Moments are
+ * 2^((c >> 3) + b - 127), 0 is zero (whatever its sign bit); code 127 of the first moment is NaN, 255 of the second infinity; finite
+ * values above 1.875 * 2^127 count as that.  All-zero arrays are the state before the first step.  Moments are
  * rounded stochastically: with mix(x) = { x ^= x >> 16; x *= 0x7FEB352D; x ^= x >> 15; x *= 0x846CA68B; x ^= x >> 16 } and L = the eight odd words of lane_word (adamw.hip),
  * element j of the tensor at place[k] (HOST int[n]; NULL: k) takes the halves of mix((j >> 3) ^ mix(seed + step * 0x9E3779B1 + place * 0x85EBCA6B)) * L[j & 7]: the same
  * seed, step and place give the same bits.  The device form takes no row_freeze; with live_rows, the rows behind them hold zero codes (they share the last live block's

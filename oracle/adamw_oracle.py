@@ -52,13 +52,15 @@ def encode(m, v, um, uv):
     um, uv = blocks_of(um.astype(np.int64)), blocks_of(uv.astype(np.int64))
     base = lambda b, below: np.maximum((np.where(b < 0x7F800000, b, 0).max(1, keepdims=True) >> 23) - below, 1)   # noqa: E731
     bm, bv = base(mb, 14), base(vb, 30)
+    m_out, v_out = mb >= 0x7F800000, vb >= 0x7F800000
+    mb, vb = np.minimum(mb, 0x7F700000), np.minimum(vb, 0x7F700000)      # 1.875 * 2^127, the last finite code of any base: larger ones do not round up to infinity
     a = mb.astype(np.uint32).view(np.float32)
     low = ((bm << 23) + (1 << 20)).astype(np.uint32).view(np.float32)
     rounded = ((mb + (um << 4) + 8) >> 20) - (bm << 3)
     mc = np.where(a < low, (a > (low * np.float32(2.0 ** -16)) * (um.astype(np.float32) + np.float32(0.5))).astype(np.int64), rounded)
-    mc = np.where(mb >= 0x7F800000, 127, mc | sign << 7)                # a zero may carry a sign: it stands for zero all the same
+    mc = np.where(m_out, 127, mc | sign << 7)                # a zero may carry a sign: it stands for zero all the same
     vc = np.maximum(((vb + (uv << 4) + 8) >> 20) - (bv << 3), 1)
-    vc = np.where(vb == 0, 0, np.where(vb >= 0x7F800000, 255, vc))
+    vc = np.where(vb == 0, 0, np.where(v_out, 255, vc))
     return (mc | vc << 8).reshape(-1)[:n].astype(np.uint16), (bm | bv << 8).reshape(-1).astype(np.uint16)
 
 

@@ -71,6 +71,10 @@ def test_ends_of_the_range():
     assert exps[0] == (240 | 224 << 8) and (codes[4:] == 0).all()
     assert abs(b[0] / float(v[0]) - 1) <= 1 / 8 and b[1] == b[2] == 1.125 * 2.0 ** 97 and np.isinf(b[3])         # above zero stays above zero
     assert abs(a[0] / float(m[0]) - 1) <= 1 / 8 and np.isnan(a[1]) and np.isnan(a[2]) and a[3] == 0
+    for k in range(64):          # never rounded up to infinity
+        c, e = ao.encode(m, v, *ao.random_bits(n, k, 1, 0))
+        a, b = ao.decode(c, e, np.float32)
+        assert np.isfinite(a[0]) and np.isfinite(b[0])
     codes, exps = ao.encode(np.zeros(n, dtype=np.float32), np.full(n, 1e-45, dtype=np.float32), *u)
     assert exps[0] == (1 | 1 << 8) and (codes == 1 << 8).all()
 

@@ -159,6 +159,7 @@ def test_wide_range_inside_a_block_of_8_bit_moments():
     g[384:512] = np.float32(1e-42)                       # subnormal gradients
     g[512:640] = -0.0
     g[640] = 3e38                                        # its square is infinite, the gradient is not
+    g[768:896] = 5.8e20                                  # squares that come near the largest float: they must not round up to infinity
     p, gd = torch.ones(n, device="cuda"), torch.from_numpy(g).cuda()
     mo, be = torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(n // 128, dtype=torch.int16, device="cuda")
     m, v = np.zeros(n, dtype=np.float32), np.zeros(n, dtype=np.float32)
@@ -168,7 +169,35 @@ def test_wide_range_inside_a_block_of_8_bit_moments():
         codes, exps = ao.encode(m32, v32, *ao.random_bits(n, 4, t, 0))
         assert np.array_equal(mo.cpu().numpy().view(np.uint16), codes) and np.array_equal(be.cpu().numpy().view(np.uint16), exps), t
         m, v = ao.decode(codes, exps, np.float32)
+        if t == 1:                                       # moments at the end of the range themselves
+            m[900], v[900] = -3.4e38, 3.4e38
+            codes, exps = ao.encode(m, v, *ao.random_bits(n, 9, 1, 0))
+            mo.copy_(torch.from_numpy(codes.view(np.int16)))
+            be.copy_(torch.from_numpy(exps.view(np.int16)))
+            m, v = ao.decode(codes, exps, np.float32)
+            assert np.isfinite(m).all() and np.isfinite(v[np.arange(n) != 640]).all()
     assert bool(torch.isfinite(p).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-15])
+def test_subnormal_second_moments(bits, eps):
+    """The hardware's square root takes subnormals for zero: with eps = 0 the update would be infinite."""
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit
+    n = 600
+    g = (1e-19 * np.linspace(0.5, 2.0, n)).astype(np.float32)           # (1 - b2) g^2 is around 1e-41
+    g[300:] = 1.0                                                       # and an ordinary half
+    p, gd = torch.zeros(n, device="cuda"), torch.from_numpy(g).cuda()
+    if bits == 32:
+        s = [torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")]
+        adamw_step([p], [gd], [s[0]], [s[1]], lr=1e-2, step=1, eps=eps)
+    else:
+        s = [torch.zeros(n, dtype=torch.int16, device="cuda"), torch.zeros(5, dtype=torch.int16, device="cuda")]
+        adamw_step_8bit([p], [gd], [s[0]], [s[1]], lr=1e-2, step=1, eps=eps)
+    m, v = (x.astype(np.float64) for x in ao.step32(np.zeros(n), np.zeros(n), g, (0.9, 0.999)))
+    assert (v[:300] < 2.0 ** -126).all() and (v > 0).all()
+    want = -1e-2 / 0.1 * m / (np.sqrt(v) / np.sqrt(1e-3) + eps)         # from the float32 moments as they are: root, its constant, sum, reciprocal, step size, two products
+    assert (np.abs(_np(p.cpu()) - want) <= 12 * 2.0 ** -24 * np.abs(want)).all()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -736,6 +765,56 @@ def test_captured_mapper_iteration_takes_it(bits, max_norm, monkeypatch):
         assert all(torch.equal(a[n], b[n]) for n in a)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_one_capture_over_a_map_that_grows_and_is_pruned(bits, monkeypatch):
+    """A stable store with FusedAdamW under ONE captured graph; sparse gradients and the step bump in the loss against the dense, separately bumped form."""
+    from diff_gaussian_rasterization import GaussianRasterizer
+    from gs_icp_slam_amd.gaussian_store import GaussianStore
+    from gs_icp_slam_amd.graph import MapperIterationGraph
+    from gs_icp_slam_amd.optim import FusedAdamW
+    P, W, H = 20000, 320, 200
+    cfg = dict(synth.REPLICA)
+    cam = synth.make_camera(W, H, cfg["fx"] * W / cfg["W"], cfg["fy"] * H / cfg["H"], synth.DEFAULT_POSE_A)
+    g = synth.s_map(P, seed=5)
+    rows = {"xyz": torch.from_numpy(g["means3D"]), "f_dc": torch.from_numpy(g["shs"]).reshape(P, 1, 3), "f_rest": torch.zeros(P, 0, 3), "scaling": torch.log(torch.from_numpy(g["scales"])),
+            "opacity": torch.logit(torch.from_numpy(g["opacities"]).clamp(1e-4, 1 - 1e-4)).reshape(P, 1), "rotation": torch.from_numpy(g["rotations"])}
+    rs = make_settings(cam, [0.0, 0.0, 0.0])
+    t2 = torch_inputs(synth.s_map(P, seed=5, perturb_seed=7))
+    with torch.no_grad():
+        depth, color, _, _ = GaussianRasterizer(rs)(means3D=t2["means3D"], means2D=torch.zeros_like(t2["means3D"]), shs=t2["shs"], opacities=t2["opacities"],
+                                                    scales=t2["scales"], rotations=t2["rotations"])
+    res = []
+    for fast in (True, False):
+        for k in ("GSICP_SPARSE_GRADS", "GSICP_STEP_BUMP_IN_LOSS"):
+            monkeypatch.setenv(k, "1" if fast else "0")
+        store = GaussianStore(P + 1000, n_rest=0, stable=True, moment_bits=bits)
+        some = lambda a, b: {k: v[a:b].cuda() for k, v in rows.items()}      # noqa: E731
+        store.append(some(0, 12345))
+        opt = store.attach(FusedAdamW, LRS, lr=0.0, eps=1e-15, weight_decay=1e-3, capturable=True, state_bits=bits, seed=1)
+        params = dict(means3D=store.params["xyz"], shs=store.params["f_dc"], opacities=store.params["opacity"], scales=store.params["scaling"], rotations=store.params["rotation"])
+        mg = MapperIterationGraph(params, opt, H, W, cam["tanfovx"], cam["tanfovy"], sh_degree=0, capacity=2_000_000, warmup=2, live_count=store.live_count)
+        mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+        mg.capture()
+        losses, before = [], None
+        for op in ("step", "step", "grow", "step", "prune", "step", "step"):
+            if op == "grow":
+                store.append(some(12345, P))
+            elif op == "prune":
+                before = store.n
+                store.prune((torch.arange(store.n, device="cuda") * 2654435761 >> 7) % 5 == 0)
+                assert 0.7 * before < store.n < 0.9 * before
+            else:
+                mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+                losses.append(float(mg.step()))
+                torch.cuda.synchronize()
+        assert not mg.overflowed() and all(np.isfinite(losses)) and int(opt.state[store.params["xyz"]]["step"]) == 5
+        res.append((losses, {k: store.live(k).clone() for k in NAMES}, {(r, k): store.view(r, k).clone() for k in NAMES for r in (("m", "v") if bits == 32 else ("c", "x"))}))
+        mg.release()
+    assert res[0][0] == res[1][0]
+    for a, b in zip(res[0][1:], res[1][1:]):
+        assert all(torch.equal(a[k], b[k]) for k in a)
+
+
 def test_a_run_of_the_operators_together():
     """Norm, 8-bit step, decode, 32-bit step from the decoded moments: as a program uses them that moves from 8-bit to 32-bit moments."""
     from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, decode_moments, grad_norm, new_moments_8bit
@@ -794,6 +873,7 @@ def test_refusals_on_the_device():
             f()
             pytest.fail(f"call {k} was not refused")
     assert adamw_step([], [], [], [], **ok) is None
+    assert float(adamw_step([z(8)], [z(8) + 2], [z(8)], [z(8)], lr=np.float32(1e-3), weight_decay=torch.tensor(0.1), step=1, max_norm=float("inf"))) == np.float32(np.sqrt(32.0))
     g8 = z(8)
     adamw_step([z(8), z(8)], [g8, g8], [z(8), z(8)], [z(8), z(8)], **ok)                              # one gradient for two parameters is read twice
     opt = FusedAdamW([torch.nn.Parameter(z(8))], state_bits=8, capturable=True)

@@ -61,6 +61,17 @@ __device__ inline float4 conv4(const float v[16], const Win& win) {
     return make_float4(o[0], o[1], o[2], o[3]);
 }
 
+// Two expressions that the two-pass and the one-kernel form of the loss share, each product and sum rounded by itself (what the
+// compiler fuses would else depend on the code around them): the denominator's term of the means,
+__device__ __forceinline__ float ssim_mean_term(float mu1, float mu2, float C1) {
+#pragma clang fp contract(off)
+    return mu1 * mu1 + mu2 * mu2 + C1;
+}
+// and the three derivative maps joined
+__device__ __forceinline__ float ssim_gradient(float a0, float x, float a1, float y, float a2) {
+#pragma clang fp contract(off)
+    return a0 + 2.f * x * a1 + y * a2;
+}
 // Pass 1.  grid = (tiles_x, tiles_y, 4): z = 0..2 colour channels, z = 3 the depth L1 term (no SSIM).
 // partial[(z * n_tiles + tile) * 2 + {0,1}] = {sum of masked |diff|, sum of SSIM map} of this workgroup.
 // Register tiling: the horizontal pass makes 4 adjacent outputs from 14 staged values (4 x ds_read_b128 per array), the vertical
@@ -180,9 +191,9 @@ __global__ __launch_bounds__(256) void loss_pass1_kernel(const float* __restrict
             if (px < W && py < H) {
                 const float mu1 = mom[0][j], mu2 = mom[1][j], e11 = mom[2][j], e22 = mom[3][j], e12 = mom[4][j];
                 const float C1 = 0.01f * 0.01f, C2 = 0.03f * 0.03f;
-                const float mu1_sq = mu1 * mu1, mu2_sq = mu2 * mu2, mu12 = mu1 * mu2;
+                const float mu12 = mu1 * mu2;
                 const float a = 2.f * mu12 + C1, b = 2.f * (e12 - mu12) + C2;
-                const float c = mu1_sq + mu2_sq + C1, d = (e11 - mu1_sq) + (e22 - mu2_sq) + C2;
+                const float c = ssim_mean_term(mu1, mu2, C1), d = __builtin_fmaf(-mu1, mu1, e11) + __builtin_fmaf(-mu2, mu2, e22) + C2;
                 // v_rcp_f32 (1 ulp) instead of IEEE divisions (~10 instructions each): c, d >= C1, C2 > 0, far from the denormal range
                 const float inv_d = __builtin_amdgcn_rcpf(d);
                 const float inv_cd = __builtin_amdgcn_rcpf(c) * inv_d;
@@ -368,7 +379,7 @@ __global__ __launch_bounds__(256) void loss_pass2_kernel(const float* __restrict
             float gr = 0.f;
             if (yv != 0.f) {
                 const float xv = HOIST ? h_im[j] : image[ch * HW + pix];
-                gr = acc[0][j] + 2.f * xv * acc[1][j] + yv * acc[2][j];
+                gr = ssim_gradient(acc[0][j], xv, acc[1][j], yv, acc[2][j]);
                 gr += xv > yv ? l1_scale : (xv < yv ? -l1_scale : 0.f);
             }
             dL_dimage[ch * HW + pix] = gr;
@@ -527,9 +538,9 @@ __global__ __launch_bounds__(256) void loss_fused_kernel(const float* __restrict
                 const bool in = qx >= 0 && qx < W && qy >= 0 && qy < H;
                 const float mu1 = mom[k][0][j], mu2 = mom[k][1][j], e11 = mom[k][2][j], e22 = mom[k][3][j], e12 = mom[k][4][j];
                 const float C1 = 0.01f * 0.01f, C2 = 0.03f * 0.03f;
-                const float mu1_sq = mu1 * mu1, mu2_sq = mu2 * mu2, mu12 = mu1 * mu2;
+                const float mu12 = mu1 * mu2;
                 const float a = 2.f * mu12 + C1, b = 2.f * (e12 - mu12) + C2;
-                const float c = mu1_sq + mu2_sq + C1, d = (e11 - mu1_sq) + (e22 - mu2_sq) + C2;
+                const float c = ssim_mean_term(mu1, mu2, C1), d = __builtin_fmaf(-mu1, mu1, e11) + __builtin_fmaf(-mu2, mu2, e22) + C2;
                 const float inv_d = __builtin_amdgcn_rcpf(d);
                 const float inv_cd = __builtin_amdgcn_rcpf(c) * inv_d;
                 const float S = a * b * inv_cd;
@@ -572,7 +583,7 @@ __global__ __launch_bounds__(256) void loss_fused_kernel(const float* __restrict
                 float gr = 0.f;
                 if (yc[j] != 0.f) {
                     l1 += fabsf(xc[j] - yc[j]);
-                    gr = acc[0][j] + 2.f * xc[j] * acc[1][j] + yc[j] * acc[2][j];
+                    gr = ssim_gradient(acc[0][j], xc[j], acc[1][j], yc[j], acc[2][j]);
                     gr += xc[j] > yc[j] ? l1_scale : (xc[j] < yc[j] ? -l1_scale : 0.f);
                 }
                 if (dL_dimage) dL_dimage[ch * HW + (size_t)py * W + px] = gr;
@@ -719,6 +730,18 @@ __device__ inline AdamPMV adam_update(float p, float m, float v, float g, float 
     o.p = p - step_size * (o.m / denom);
     return o;
 }
+// the elements behind the last whole 16 bytes: the second moment's products and sum rounded one by one (elsewhere the last product is fused into the sum)
+__device__ inline AdamPMV adam_update_tail(float p, float m, float v, float g, float beta1, float beta2, float eps, float inv_bc2_sqrt, float step_size) {
+    AdamPMV o;
+    o.m = __builtin_fmaf(1.f - beta1, g - m, m);
+    {
+#pragma clang fp contract(off)
+        o.v = beta2 * v + (1.f - beta2) * g * g;
+    }
+    const float denom = __builtin_fmaf(sqrtf(o.v), inv_bc2_sqrt, eps);
+    o.p = __builtin_fmaf(-step_size, o.m / denom, p);
+    return o;
+}
 // torch.optim.Adam (amsgrad off, weight decay 0, maximize off):  m += (1-b1)(g-m);  v = b2 v + (1-b2) g g;
 // p -= step_size * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // grid = (x, tensor): blockIdx.y picks the tensor, so no per-element group lookup, and each lane moves 16 bytes per access (the update
@@ -800,7 +823,7 @@ __device__ __forceinline__ void adam_tensor_body(const AdamTable& t, const doubl
         for (long long j = 4 * nvec + (long long)blockIdx.x * 256 + threadIdx.x; j < numel; j += stride) {
             const unsigned row = (unsigned)j / gw;
             if (rw && row_freeze[row] != 0) continue;
-            const AdamPMV a0 = adam_update(P[j], M[j], V[j], grad_rows[row] > 0 ? G[j] : 0.f, beta1, beta2, eps, inv_bc2_sqrt, step_size);
+            const AdamPMV a0 = adam_update_tail(P[j], M[j], V[j], grad_rows[row] > 0 ? G[j] : 0.f, beta1, beta2, eps, inv_bc2_sqrt, step_size);
             M[j] = a0.m; V[j] = a0.v; P[j] = a0.p;
         }
         return;
@@ -825,7 +848,7 @@ __device__ __forceinline__ void adam_tensor_body(const AdamTable& t, const doubl
     }
     for (long long j = 4 * nvec + (long long)blockIdx.x * 256 + threadIdx.x; j < numel; j += stride) {
         if (rw && row_freeze[(unsigned)j / rw] != 0) continue;
-        const AdamPMV a0 = adam_update(P[j], M[j], V[j], G[j], beta1, beta2, eps, inv_bc2_sqrt, step_size);
+        const AdamPMV a0 = adam_update_tail(P[j], M[j], V[j], G[j], beta1, beta2, eps, inv_bc2_sqrt, step_size);
         M[j] = a0.m; V[j] = a0.v; P[j] = a0.p;
     }
 }

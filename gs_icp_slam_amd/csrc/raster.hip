@@ -934,7 +934,11 @@ __global__ __launch_bounds__(256) void blend_backward_tile_kernel(BlendArgs a) {
         dp0 = a.dL_dpix[pix]; dp1 = a.dL_dpix[HW + pix]; dp2 = a.dL_dpix[2 * HW + pix];
         dpd = a.dL_ddepth ? a.dL_ddepth[pix] : 0.f;
     }
-    float bg_dot = a.bg[0] * dp0 + a.bg[1] * dp1 + a.bg[2] * dp2;
+    float bg_dot;
+    {   // the first product is fused into its sum; the other two are rounded
+#pragma clang fp contract(off)
+        bg_dot = __builtin_fmaf(a.bg[0], dp0, a.bg[1] * dp1) + a.bg[2] * dp2;
+    }
     if (a.depth_mode == 1) {
         // D = N / A with A = 1 - T_final:  dD/dalpha_i = (dN/dalpha_i) / A - (N / A^2) T_final / (1 - alpha_i).  The first term is the
         // un-normalised rule fed with dL/dD / A; the second has exactly the form of the background term (-T_final / (1 - alpha_i) * x).

@@ -7,7 +7,7 @@
 // One rule (a character) and one name (for the errors) per list; the first list has rule 'p' or 'c' and says device, length and element counts:
 //   p  float32 / bfloat16 / float16 (their codes are recorded)      g  the first list's dtype, read only      f  float32         h  int16
 //   b  int16, one element per 128 of the first list's               m  float32 or None                        c  int16 (as p, codes 0)
-// At `address` (kept alive by `keep`): for each list n 8-byte addresses (0 for None and for empty tensors), then n int64 element counts, then n int32 codes.
+// At `address` (kept alive by `keep`, which holds the lists too): for each list n 8-byte addresses (0 for None and for empty tensors), then n int64 element counts, then n int32 codes.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -105,7 +105,11 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         }
         const unsigned long long stream = (unsigned long long)(uintptr_t)c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
         PyObject* current = c10::hip::current_device() == device ? Py_True : Py_False;
-        return Py_BuildValue("(iOKnKN)", device, current, stream, n, (unsigned long long)(uintptr_t)base, keep);
+        PyObject* alive = PyTuple_New(1 + lists);      // also the tensors that an iterator has made: nothing else may hold them
+        if (!alive) { Py_DECREF(keep); return nullptr; }
+        PyTuple_SET_ITEM(alive, 0, keep);
+        for (int l = 0; l < lists; ++l) { Py_INCREF(refs.seq[l]); PyTuple_SET_ITEM(alive, 1 + l, refs.seq[l]); }
+        return Py_BuildValue("(iOKnKN)", device, current, stream, n, (unsigned long long)(uintptr_t)base, alive);
     } catch (const std::exception& e) {
         Py_XDECREF(keep);
         PyErr_SetString(PyExc_RuntimeError, e.what());

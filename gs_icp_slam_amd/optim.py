@@ -261,7 +261,7 @@ _tensor_lists = None
 
 def _pack(what, names, rules, *lists):
     """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, whether it is the current one, its current stream, n, address of the arrays, what
-    keeps them alive).  The arrays: n addresses per list, n element counts (8 bytes each), n dtype codes."""
+    keeps them and the tensors alive).  The arrays: n addresses per list, n element counts (8 bytes each), n dtype codes."""
     global _tensor_lists
     if _tensor_lists is None:
         try:
@@ -537,6 +537,8 @@ class FusedAdamW(FusedAdam):
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW: sparse gradients are not supported")
                 st = self.state[p]
+                if self.capturable and not torch.is_tensor(st.get("step")) and torch.cuda.is_current_stream_capturing():      # state made now would live in the graph, unwritten
+                    raise RuntimeError("FusedAdamW(capturable): run one step() outside graph capture first (allocates the state)")
                 if not st:
                     if self.capturable and p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.int32, device=p.device)

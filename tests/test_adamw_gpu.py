@@ -893,3 +893,43 @@ def test_refusals_on_the_device():
         with pytest.raises(RuntimeError):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 o.step()
+
+
+def test_a_refused_capture_leaves_the_optimiser_as_it_was():
+    """Neither a first step nor the first one after loading host step counts can be captured; an eager step afterwards starts from where the state stood."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    for first_steps in (0, 2):
+        host, dev = _params(9), _params(9)
+        a, b = FusedAdamW(host, lr=1e-2), FusedAdamW(dev, lr=1e-2, capturable=True)
+        for k in range(first_steps):
+            _feed(host, k)
+            a.step()
+        for p, q in zip(host, dev):
+            q.data.copy_(p)
+            if first_steps:
+                b.state[q].update({name: v.clone() if torch.is_tensor(v) else v for name, v in a.state[p].items()})
+        _feed(host, 7)
+        _feed(dev, 7)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside graph capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                b.step()
+        assert all(b.state[q].get("step", 0) == first_steps for q in dev)
+        a.step()
+        b.step()
+        for p, q in zip(host, dev):
+            assert torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"]) and torch.equal(a.state[p]["exp_avg_sq"], b.state[q]["exp_avg_sq"])
+            assert int(b.state[q]["step"]) == first_steps + 1 == a.state[p]["step"]
+
+
+def test_tensors_that_only_an_iterator_holds():
+    """Lists may be iterators that make their tensors: these live until the kernels are launched (the norm's workspace must not come to lie over them)."""
+    from gs_icp_slam_amd.optim import adamw_step, grad_norm
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    base = [torch.randn(n, device="cuda", generator=gen) for n in (300_000, 300_000, 1000)]
+    assert torch.equal(grad_norm(t * 2 for t in base), grad_norm([t * 2 for t in base]))
+    new = lambda: [torch.zeros_like(t) for t in base]                 # noqa: E731
+    x, y = (new(), new(), new()), (new(), new(), new())
+    n1 = adamw_step(x[0], (t * 2 for t in base), x[1], x[2], lr=1e-2, step=1, max_norm=0.5)
+    n2 = adamw_step(y[0], [t * 2 for t in base], y[1], y[2], lr=1e-2, step=1, max_norm=0.5)
+    assert torch.equal(n1, n2) and all(torch.equal(s, t) for ls, lt in zip(x, y) for s, t in zip(ls, lt))

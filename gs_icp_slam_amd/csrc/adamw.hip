@@ -36,7 +36,7 @@ namespace {
 
 constexpr int TABLE = 64;             // tensors per launch: the table travels in the kernel arguments (< 4 KB), nothing is copied or kept
 constexpr int DEV_TABLE = 56;         // with what the device form adds
-constexpr int NORM_TABLE = 128;
+constexpr int NORM_TABLE = 240;
 constexpr uint32_t LAST = 0x7FFFFFFF; // a tile number that no launch reaches
 constexpr long long MAX_NUMEL = 1ll << 33;   // 2^25 workgroups of the step for one tensor; a launch has less than 2^32 lanes
 constexpr unsigned long long STEP_TILES = (1u << 26) - 1, DECODE_TILES = (1u << 24) - 1;
@@ -577,8 +577,19 @@ __global__ __launch_bounds__(64) void adamw_gather_kernel(GatherTable t, const l
 // Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split, and the squares of large
 // or small f32 gradients would leave its range.  The sums are split over the workgroups by position alone and joined in a fixed order.
 // Measured: 133 M f16 gradients 42 us = 6.4 TB/s and 4.7 us for the join of 2 048 sums, 45 as calls follow each other (with 1 024 workgroups 53); 4.2 M f32 ones 4.8 + 2.2 us.
-struct NormEntry { const void* g; long long numel; int dtype, pad; };
-struct NormTable { uint32_t first[NORM_TABLE]; NormEntry e[NORM_TABLE]; };
+struct NormEntry { const void* g; long long numel; int dtype; };
+struct NormTable {      // 16 bytes a tensor: 240 of them in one launch (128 in entries of 28: 200 tensors of 7 and 12 elements 17.3 us, so 14.3; 400 of them 26.9 and 18.0)
+    uint32_t first[NORM_TABLE];
+    struct { uint32_t at_low, at_high, numel_low; } e[NORM_TABLE];      // 58 bits address, 2 bits Dtype, the rest of numel
+    __host__ void set(int k, const void* g, long long numel, int dtype) {
+        const uint64_t at = (uint64_t)(uintptr_t)g | (uint64_t)dtype << 58 | (uint64_t)numel >> 32 << 60;
+        e[k] = {(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)numel};
+    }
+    __device__ __forceinline__ NormEntry entry(uint32_t k) const {
+        const uint64_t at = (uint64_t)e[k].at_high << 32 | e[k].at_low;
+        return {(const void*)(at & ((1ull << 58) - 1)), (long long)(at >> 60 << 32 | e[k].numel_low), (int)(at >> 58 & 3u)};
+    }
+};
 static_assert(sizeof(NormTable) + 64 <= 4096, "kernel arguments of a launch");
 
 __host__ __device__ constexpr int norm_tile_elems(int dtype, int bytes) { return bytes / (dtype == F32 ? 4 : 2); }
@@ -624,7 +635,7 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
 template <bool NT>
 __device__ __forceinline__ double norm_any_tile(const NormTable& t, uint32_t tile, int lanes, int lane) {
     const uint32_t k = find_tensor(t.first, tile);
-    const NormEntry& e = t.e[k];
+    const NormEntry e = t.entry(k);
     const uint32_t mine = tile - t.first[k];
     return e.dtype == F32 ? norm_tile<F32, NT>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16, NT>(e, mine, lanes, lane) : norm_tile<F16, NT>(e, mine, lanes, lane);
 }
@@ -944,6 +955,7 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
         if (numel[k] < 0 || numel[k] > MAX_NUMEL) return fail("gsicp_grad_norm: a tensor has 0 to 2^33 elements");
         if (numel[k] == 0) continue;
         if (!grads[k] || dtype[k] < F32 || dtype[k] > F16) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
+        if ((uint64_t)(uintptr_t)grads[k] >> 58) return fail("gsicp_grad_norm: an address has less than 2^58");
     }
     const bool one = norm_is_small(n, numel, dtype);
     if (!one && !scratch) return fail("gsicp_grad_norm: missing scratch");
@@ -956,7 +968,7 @@ int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, con
         unsigned long long tiles = 0;
         for (; k < n && m < NORM_TABLE; ++k) {
             if (numel[k] == 0) continue;
-            t.e[m] = {grads[k], numel[k], dtype[k], 0};
+            t.set(m, grads[k], numel[k], dtype[k]);
             t.first[m++] = (uint32_t)tiles;
             const int te = norm_tile_elems(dtype[k], tile_bytes);
             tiles += (unsigned long long)((numel[k] + te - 1) / te);       // at most 2^21 of one tensor

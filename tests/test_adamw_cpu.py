@@ -156,10 +156,11 @@ def test_c_abi_refuses_before_it_launches():
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(0), 0.0, None, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(5), (ctypes.c_int * 1)(5), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(0), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
+    assert lib.gsicp_grad_norm(1, one(1 << 58), k(5), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k((1 << 33) + 1), (ctypes.c_int * 1)(0), 0.0, 64, 64, 64, None) == -2
     assert lib.gsicp_grad_norm(1, one(64), k(1 << 30), (ctypes.c_int * 1)(0), 0.0, 64, 64, None, None) == -2          # a large set needs its scratch
     size = lambda n, each: lib.gsicp_grad_norm_scratch_bytes(n, (ctypes.c_longlong * n)(*[each] * n), (ctypes.c_int * n)(*[0] * n))      # noqa: E731
-    assert size(1, 5) == size(64, 7) == 0 and size(65, 7) == size(1, 1 << 30) > 0 and size(129, 7) > size(128, 7)
+    assert size(1, 5) == size(64, 7) == 0 and size(65, 7) == size(1, 1 << 30) > 0 and size(241, 7) > size(240, 7)
 
 
 def test_python_layer_has_no_cpu_path_and_refuses_bad_options():

@@ -327,7 +327,7 @@ def test_gathered_rows_of_8_bit_moments(rows, widths):
 
 
 # ------------------------------------------------------------------------------------------------ global norm
-@pytest.mark.parametrize("sizes", [[1], [0], [0, 0, 3], MANY, [7, 12] * 100, [3_000_001, 5]])
+@pytest.mark.parametrize("sizes", [[1], [0], [0, 0, 3], MANY, [7, 12] * 100, [5, 0, 700] * 80, [7, 12, 9000] * 81, [3_000_001, 5]])
 def test_grad_norm_over_mixed_types(sizes):
     from gs_icp_slam_amd.optim import grad_norm
     rng = np.random.default_rng(len(sizes))

@@ -81,6 +81,7 @@ SIGNATURES = {
     "gsicp_adamw_gather_rows": (c_int, [c_int] + [c_void_p] * 6 + [ctypes.c_longlong, ctypes.c_longlong, c_void_p]),
     "gsicp_grad_norm_scratch_bytes": (c_size_t, [c_int, c_void_p, c_void_p]),
     "gsicp_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gsicp_grad_norm_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gsicp_stream_create_cu_mask": (c_void_p, [c_int, c_int]),
     "gsicp_stream_destroy": (c_int, [c_void_p]),
     "gsicp_gicp_create": (c_void_p, []),

@@ -37,6 +37,7 @@ namespace {
 constexpr int TABLE = 64;             // tensors per launch: the table travels in the kernel arguments (< 4 KB), nothing is copied or kept
 constexpr int DEV_TABLE = 56;         // with what the device form adds
 constexpr int NORM_TABLE = 240;
+constexpr int NORM_ROWS_TABLE = 120;  // with rows that are left out
 constexpr uint32_t LAST = 0x7FFFFFFF; // a tile number that no launch reaches
 constexpr long long MAX_NUMEL = 1ll << 33;   // 2^25 workgroups of the step for one tensor; a launch has less than 2^32 lanes
 constexpr unsigned long long STEP_TILES = (1u << 26) - 1, DECODE_TILES = (1u << 24) - 1;
@@ -312,7 +313,16 @@ struct Rows {
         const uint32_t t = __umulhi(magic, n);
         return width == 1u ? n : (t + ((n - t) >> 1)) >> shift;
     }
+    // rows of the elements at ... at + nv - 1, those behind them as the first: at most two rows when a row has three elements or more
+    __device__ __forceinline__ void of4(uint32_t at, int nv, uint32_t row[4]) const {
+        const uint32_t w = width, first = of(at), col = at - first * w, last = of(at + (uint32_t)max(nv, 1) - 1u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row[j] = w >= 3u ? (col + j < w ? first : last) : (w == 2u ? (at + j) >> 1 : at + j);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) row[j] = j < nv ? row[j] : row[0];
+    }
 };
+__device__ __forceinline__ uint32_t row_shift(uint32_t w) { return w > 1u ? 31u - __builtin_clz(w - 1u) : 0u; }
 // one bit per element: word > 0 (kind 0) or word == 0 (kind 1)
 __device__ __forceinline__ uint32_t row_flag(int word, int kind) { return kind == 0 ? (word > 0 ? 1u : 0u) : (word == 0 ? 1u : 0u); }
 __device__ __forceinline__ uint32_t flags4(const int* words, const uint32_t row[4], int kind) {
@@ -348,15 +358,11 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
     if (!MASKED || rows.width == 0) {
         load4<DT, FULL, NT>(e.g, at, nv, g);
     } else {
-        // The rows of the four elements are at most two when a row has three elements or more: two words to read, not four.  With the division by multiplication and the gradient
+        // Two words to read where the four elements are of two rows, not four.  With the division by multiplication and the gradient
         // not read where all four are culled, 23.0 -> 20.8 us for 4.2 M elements of 300 k rows.
-        const uint32_t w = rows.width, first = rows.of((uint32_t)at), col = (uint32_t)at - first * w;
-        const uint32_t last_row = rows.of((uint32_t)at + (uint32_t)max(nv, 1) - 1u);
+        const uint32_t w = rows.width;
         uint32_t row[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) row[j] = w >= 3u ? (col + j < w ? first : last_row) : (w == 2u ? ((uint32_t)at + j) >> 1 : (uint32_t)at + j);
-#pragma unroll
-        for (int j = 1; j < 4; ++j) row[j] = FULL || j < nv ? row[j] : row[0];
+        rows.of4((uint32_t)at, nv, row);
         uint32_t live = 0xFu;
         if (FULL || nv > 0) {
             if (rows.grad) live = w >= 3u ? flags2(rows.grad, row, 0) : flags4(rows.grad, row, 0);
@@ -457,7 +463,7 @@ __global__ __launch_bounds__(64) void adamw_step_kernel(StepTable<DEV> t, StepHy
     if constexpr (DEV) {
         if (h.guard_count && *h.guard_count > h.guard_limit) return;      // the iteration that made these gradients is void: nothing moves
         rows.width = t.row_width[k];
-        if (MASKED) { rows.magic = t.row_magic[k]; rows.shift = rows.width > 1u ? 31u - __builtin_clz(rows.width - 1u) : 0u; }
+        if (MASKED) { rows.magic = t.row_magic[k]; rows.shift = row_shift(rows.width); }
         if (h.live_rows && rows.width > 0) numel = min(numel, (long long)*h.live_rows * rows.width);     // rows behind the live count are not parameters
         step += *h.step_dev;
         const double lr = h.lr_dev[h.src + k];
@@ -542,7 +548,7 @@ static_assert(sizeof(GatherTable) + 64 <= 4096, "kernel arguments of a launch");
 __global__ __launch_bounds__(64) void adamw_gather_kernel(GatherTable t, const long long* __restrict__ index, uint32_t n_rows, long long src_rows) {
     const uint32_t k = find_tensor(t.first, blockIdx.x), mine = blockIdx.x - t.first[k];
     const GatherEntry e = t.e[k];
-    const Rows rows = {e.width, e.magic, e.width > 1u ? 31u - __builtin_clz(e.width - 1u) : 0u, nullptr, nullptr};
+    const Rows rows = {e.width, e.magic, row_shift(e.width), nullptr, nullptr};
     const uint32_t numel = n_rows * e.width, at = mine * TILE_ELEMS + 4 * threadIdx.x;       // below 2^32 (checked on the host)
     uint32_t am[4], av[4], sign[4], tm = 0, tv = 0;      // code + 8 base; 0: zero, ~0: not finite
 #pragma unroll
@@ -577,20 +583,30 @@ __global__ __launch_bounds__(64) void adamw_gather_kernel(GatherTable t, const l
 // Squares and sums in 64 bits: 133 M f16 gradients summed in 32 would lose what the clip factor needs to be the same from run to run and split to split, and the squares of large
 // or small f32 gradients would leave its range.  The sums are split over the workgroups by position alone and joined in a fixed order.
 // Measured: 133 M f16 gradients 42 us = 6.4 TB/s and 4.7 us for the join of 2 048 sums, 45 as calls follow each other (with 1 024 workgroups 53); 4.2 M f32 ones 4.8 + 2.2 us.
-struct NormEntry { const void* g; long long numel; int dtype; };
-struct NormTable {      // 16 bytes a tensor: 240 of them in one launch (128 in entries of 28: 200 tensors of 7 and 12 elements 17.3 us, so 14.3; 400 of them 26.9 and 18.0)
-    uint32_t first[NORM_TABLE];
-    struct { uint32_t at_low, at_high, numel_low; } e[NORM_TABLE];      // 58 bits address, 2 bits Dtype, the rest of numel
-    __host__ void set(int k, const void* g, long long numel, int dtype) {
-        const uint64_t at = (uint64_t)(uintptr_t)g | (uint64_t)dtype << 58 | (uint64_t)numel >> 32 << 60;
-        e[k] = {(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)numel};
+struct NormEntry { const void* g; long long numel; int dtype; bool frozen; };
+struct NormPacked {      // 58 bits address, 2 bits Dtype, the rest of numel (2 bits), 1 bit: rows may be frozen
+    uint32_t at_low, at_high, numel_low;
+    __host__ void set(const void* g, long long numel, int dtype, bool frozen) {
+        const uint64_t at = (uint64_t)(uintptr_t)g | (uint64_t)dtype << 58 | (uint64_t)numel >> 32 << 60 | (uint64_t)frozen << 62;
+        *this = {(uint32_t)at, (uint32_t)(at >> 32), (uint32_t)numel};
     }
-    __device__ __forceinline__ NormEntry entry(uint32_t k) const {
-        const uint64_t at = (uint64_t)e[k].at_high << 32 | e[k].at_low;
-        return {(const void*)(at & ((1ull << 58) - 1)), (long long)(at >> 60 << 32 | e[k].numel_low), (int)(at >> 58 & 3u)};
+    __device__ __forceinline__ NormEntry entry() const {
+        const uint64_t at = (uint64_t)at_high << 32 | at_low;
+        return {(const void*)(at & ((1ull << 58) - 1)), (long long)((at >> 60 & 3u) << 32 | numel_low), (int)(at >> 58 & 3u), (at >> 62 & 1u) != 0};
     }
 };
-static_assert(sizeof(NormTable) + 64 <= 4096, "kernel arguments of a launch");
+template <bool ROWS> struct NormTable;
+template <> struct NormTable<false> {      // 16 bytes a tensor: 240 of them in one launch (128 in entries of 28: 200 tensors of 7 and 12 elements 17.3 us, so 14.3; 400 of them 26.9 and 18.0)
+    uint32_t first[NORM_TABLE];
+    NormPacked e[NORM_TABLE];
+};
+template <> struct NormTable<true> {       // rows behind a live count and frozen rows are no parameters: their gradients do not count, whatever they hold
+    uint32_t first[128];
+    NormPacked e[NORM_ROWS_TABLE];
+    uint32_t row_width[NORM_ROWS_TABLE], row_magic[NORM_ROWS_TABLE];   // as in StepTable<true>
+    const int *live_rows, *row_freeze;
+};
+static_assert(sizeof(NormTable<false>) + 64 <= 4096 && sizeof(NormTable<true>) + 64 <= 4096, "kernel arguments of a launch");
 
 __host__ __device__ constexpr int norm_tile_elems(int dtype, int bytes) { return bytes / (dtype == F32 ? 4 : 2); }
 
@@ -632,11 +648,38 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
     }
     return s;
 }
-template <bool NT>
-__device__ __forceinline__ double norm_any_tile(const NormTable& t, uint32_t tile, int lanes, int lane) {
+// the same of an f32 tensor of less than 2^32 elements without its frozen rows
+__device__ __forceinline__ double norm_frozen_tile(const NormEntry& e, const Rows& rows, uint32_t tile, int lanes, int lane) {
+    double s = 0.0;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+        const long long at = (long long)tile * (16 * lanes) + 4 * (k * lanes + lane);
+        const int nv = (int)max(0ll, min(4ll, e.numel - at));
+        if (nv == 0) break;
+        float x[4];
+        uint32_t row[4];
+        load4<F32, false, false>(e.g, at, nv, x);
+        rows.of4((uint32_t)at, nv, row);
+        const uint32_t moves = rows.width >= 3u ? flags2(rows.freeze, row, 1) : flags4(rows.freeze, row, 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double y = moves >> j & 1u ? x[j] : 0.f;
+            s = __builtin_fma(y, y, s);
+        }
+    }
+    return s;
+}
+template <bool NT, bool ROWS>
+__device__ __forceinline__ double norm_any_tile(const NormTable<ROWS>& t, uint32_t tile, int lanes, int lane) {
     const uint32_t k = find_tensor(t.first, tile);
-    const NormEntry e = t.entry(k);
+    NormEntry e = t.e[k].entry();
     const uint32_t mine = tile - t.first[k];
+    if constexpr (ROWS) {
+        const uint32_t w = t.row_width[k];
+        if (t.live_rows && w > 0) e.numel = min(e.numel, (long long)*t.live_rows * w);
+        if ((long long)mine * norm_tile_elems(e.dtype, 64 * lanes) >= e.numel) return 0.0;
+        if (e.frozen) return norm_frozen_tile(e, {w, t.row_magic[k], row_shift(w), nullptr, t.row_freeze}, mine, lanes, lane);
+    }
     return e.dtype == F32 ? norm_tile<F32, NT>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16, NT>(e, mine, lanes, lane) : norm_tile<F16, NT>(e, mine, lanes, lane);
 }
 template <int WAVES>
@@ -660,10 +703,10 @@ __device__ __forceinline__ void norm_results(double sum, double max_norm, float*
     *norm_out = norm;
     if (clip_out) *clip_out = max_norm > 0.0 ? (float)(c > 1.0 ? 1.0 : c) : 1.f;
 }
-template <bool NT>
-__global__ __launch_bounds__(256, 8) void grad_norm_kernel(NormTable t, uint32_t tiles, double* partial) {
+template <bool NT, bool ROWS>
+__global__ __launch_bounds__(256, 8) void grad_norm_kernel(NormTable<ROWS> t, uint32_t tiles, double* partial) {
     double s = 0.0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile<NT>(t, tile, 256, threadIdx.x);
+    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) s += norm_any_tile<NT, ROWS>(t, tile, 256, threadIdx.x);
     s = block_sum<4>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -681,9 +724,10 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double* __
     if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
 }
 // few small tensors: one workgroup, a tile per WAVE, no second launch
-__global__ __launch_bounds__(1024) void grad_norm_small_kernel(NormTable t, uint32_t tiles, double max_norm, float* norm_out, float* clip_out) {
+template <bool ROWS>
+__global__ __launch_bounds__(1024) void grad_norm_small_kernel(NormTable<ROWS> t, uint32_t tiles, double max_norm, float* norm_out, float* clip_out) {
     double s = 0.0;
-    for (uint32_t tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tile < tiles; tile += 16) s += norm_any_tile<false>(t, tile, 64, threadIdx.x & 63);
+    for (uint32_t tile = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tile < tiles; tile += 16) s += norm_any_tile<false, ROWS>(t, tile, 64, threadIdx.x & 63);
     s = block_sum<16>(s);
     if (threadIdx.x == 0) norm_results(s, max_norm, norm_out, clip_out);
 }
@@ -944,51 +988,80 @@ static bool norm_is_small(int n, const long long* numel, const int* dtype) {
 }
 
 size_t gsicp_grad_norm_scratch_bytes(int n, const long long* numel, const int* dtype) {
-    return n <= 0 || !numel || !dtype || norm_is_small(n, numel, dtype) ? 0 : (size_t)((n + NORM_TABLE - 1) / NORM_TABLE) * NORM_GRID * sizeof(double);
+    return n <= 0 || !numel || !dtype || norm_is_small(n, numel, dtype) ? 0 : (size_t)((n + NORM_ROWS_TABLE - 1) / NORM_ROWS_TABLE) * NORM_GRID * sizeof(double);
 }
 
-int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
-                    void* stream_v) {
-    hipStream_t stream = (hipStream_t)stream_v;
+}  // extern "C"
+
+// ROWS: live_rows, row_width, row_freeze and group_frozen of *rows apply
+template <bool ROWS>
+static int grad_norm_call(int n, const void* const* grads, const long long* numel, const int* dtype, const gsicp_adamw_device* rows, double max_norm, float* norm_out,
+                          float* clip_out, void* scratch, hipStream_t stream) {
+    constexpr int ENTRIES = ROWS ? NORM_ROWS_TABLE : NORM_TABLE;
     if (n < 0 || (n > 0 && (!grads || !numel || !dtype)) || !norm_out) return fail("gsicp_grad_norm: missing arrays");
+    if (ROWS && n > 0 && !rows->row_width) return fail("gsicp_grad_norm: live rows and frozen rows need row_width");
+    if (ROWS && rows->row_freeze && !rows->group_frozen) return fail("gsicp_grad_norm: row_freeze needs group_frozen");
     for (int k = 0; k < n; ++k) {
         if (numel[k] < 0 || numel[k] > MAX_NUMEL) return fail("gsicp_grad_norm: a tensor has 0 to 2^33 elements");
         if (numel[k] == 0) continue;
         if (!grads[k] || dtype[k] < F32 || dtype[k] > F16) return fail("gsicp_grad_norm: null pointer, or a dtype that is not 0 (f32), 1 (bf16) or 2 (f16)");
         if ((uint64_t)(uintptr_t)grads[k] >> 58) return fail("gsicp_grad_norm: an address has less than 2^58");
+        if (ROWS && rows->row_freeze && rows->group_frozen[k] && (dtype[k] != F32 || numel[k] >= (1ll << 32)))
+            return fail("gsicp_grad_norm: frozen rows go with f32 gradients of less than 2^32 elements");
     }
-    const bool one = norm_is_small(n, numel, dtype);
+    const bool one = norm_is_small(n, numel, dtype);      // at most NORM_SMALL_TILES tensors then: one table of either kind
     if (!one && !scratch) return fail("gsicp_grad_norm: missing scratch");
     const int tile_bytes = one ? 64 * 64 : 256 * 64;
     double* partial = (double*)scratch;
     int used = 0;
     for (int k = 0; k < n || one;) {
-        NormTable t = {};
+        NormTable<ROWS> t = {};
         int m = 0;
         unsigned long long tiles = 0;
-        for (; k < n && m < NORM_TABLE; ++k) {
+        for (; k < n && m < ENTRIES; ++k) {
             if (numel[k] == 0) continue;
-            t.set(m, grads[k], numel[k], dtype[k]);
+            bool frozen = false;
+            if constexpr (ROWS) {
+                const uint32_t w = rows->row_width[k] > 0 ? (uint32_t)rows->row_width[k] : 0u;
+                t.row_width[m] = w;
+                t.row_magic[m] = w > 1 ? row_magic(w) : 0u;
+                frozen = rows->row_freeze && rows->group_frozen[k] && w > 0;
+            }
+            t.e[m].set(grads[k], numel[k], dtype[k], frozen);
             t.first[m++] = (uint32_t)tiles;
             const int te = norm_tile_elems(dtype[k], tile_bytes);
             tiles += (unsigned long long)((numel[k] + te - 1) / te);       // at most 2^21 of one tensor
         }
-        for (int i = m; i < NORM_TABLE; ++i) t.first[i] = LAST;
+        for (int i = m; i < (int)(sizeof(t.first) / sizeof(t.first[0])); ++i) t.first[i] = LAST;
+        if constexpr (ROWS) { t.live_rows = rows->live_rows; t.row_freeze = rows->row_freeze; }
         if (one) {
-            hipLaunchKernelGGL(grad_norm_small_kernel, dim3(1), dim3(1024), 0, stream, t, (uint32_t)tiles, max_norm, norm_out, clip_out);
+            hipLaunchKernelGGL((grad_norm_small_kernel<ROWS>), dim3(1), dim3(1024), 0, stream, t, (uint32_t)tiles, max_norm, norm_out, clip_out);
             break;
         }
         if (m == 0) break;
         const unsigned grid = (unsigned)std::min<unsigned long long>(tiles, NORM_GRID);
         // Before a clipped step the gradients had better stay in the memory-side cache for it (its own streams pass by): norm and step of 225 MiB of gradients 278 us, with
         // non-temporal loads here 302, of 45 MiB 61 and 66.  The norm alone is better off without: 43 and 39 us, 12.4 and 12.3.
-        if (max_norm > 0.0) hipLaunchKernelGGL((grad_norm_kernel<false>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
-        else hipLaunchKernelGGL((grad_norm_kernel<true>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
+        if (ROWS || max_norm > 0.0) hipLaunchKernelGGL((grad_norm_kernel<false, ROWS>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
+        else hipLaunchKernelGGL((grad_norm_kernel<!ROWS, ROWS>), dim3(grid), dim3(256), 0, stream, t, (uint32_t)tiles, partial + used);
         used += (int)grid;
     }
     if (!one) hipLaunchKernelGGL(grad_norm_finish_kernel, dim3(1), dim3(1024), 0, stream, (const double*)partial, used, max_norm, norm_out, clip_out);
     if (hipGetLastError() != hipSuccess) { g_last_error = "gsicp_grad_norm: kernel launch failed"; return -1; }
     return 0;
+}
+
+extern "C" {
+
+int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
+                    void* stream) {
+    return grad_norm_call<false>(n, grads, numel, dtype, nullptr, max_norm, norm_out, clip_out, scratch, (hipStream_t)stream);
+}
+
+int gsicp_grad_norm_rows(int n, const void* const* grads, const long long* numel, const int* dtype, const gsicp_adamw_device* rows, double max_norm, float* norm_out,
+                         float* clip_out, void* scratch, void* stream) {
+    if (!rows || rows->grad_rows) return fail("gsicp_grad_norm_rows: rows is missing, or has gradients of which some rows were not written");
+    return grad_norm_call<true>(n, grads, numel, dtype, rows, max_norm, norm_out, clip_out, scratch, (hipStream_t)stream);
 }
 
 }  // extern "C"

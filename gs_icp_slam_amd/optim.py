@@ -301,8 +301,8 @@ def _call(name, device, current, *args):
         _lib.check(rc, name)
 
 
-def _norm(what, device, current, stream, n, addresses, numels, codes, max_norm):
-    """-> (norm: 0-dim f32 on the device, buffer whose first word is the clip factor or None)."""
+def _norm(what, device, current, stream, n, addresses, numels, codes, max_norm, rows=None):
+    """-> (norm: 0-dim f32 on the device, buffer whose first word is the clip factor or None).  rows: address of a gsicp_adamw_device that says which rows do not count."""
     dev = torch.device("cuda", device)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = _lib.load().gsicp_grad_norm_scratch_bytes(n, numels, codes)
@@ -313,7 +313,11 @@ def _norm(what, device, current, stream, n, addresses, numels, codes, max_norm):
         buffer = torch.empty(size + 8, dtype=torch.uint8, device=dev)
         clip = buffer.data_ptr()
         scratch = clip + 8
-    _call("gsicp_grad_norm", device, current, n, addresses, numels, codes, max_norm or 0.0, norm.data_ptr(), clip, scratch, stream)
+    out = (max_norm or 0.0, norm.data_ptr(), clip, scratch, stream)
+    if rows is None:
+        _call("gsicp_grad_norm", device, current, n, addresses, numels, codes, *out)
+    else:
+        _call("gsicp_grad_norm_rows", device, current, n, addresses, numels, codes, rows, *out)
     return norm, buffer
 
 
@@ -441,7 +445,8 @@ class FusedAdamW(FusedAdam):
                     8: state[p] = {"step", "moments", "block_exps"} — adamw_step_8bit's; `moments(p)` gives their values.  For a map that grows or is pruned:
                     GaussianStore(moment_bits=8)
     master_weights  16-bit parameters keep an f32 copy in state[p]["master"] that takes the update
-    max_grad_norm   clip by the global norm of all gradients of the step; `last_grad_norm` is then a 0-dim device tensor
+    max_grad_norm   clip by the global norm of all gradients of the step; `last_grad_norm` is then a 0-dim device tensor.  Rows that the step leaves alone (set_live_rows,
+                    set_row_freeze) do not count, whatever their gradients hold
     seed            of the stochastic rounding of 8-bit moments
     capturable      as in FusedAdam: step count and learning rates on the device, the step can be captured and replayed; weight decay, betas and max_grad_norm are part of the
                     capture.  MapperIterationGraph takes it wherever it takes FusedAdam."""
@@ -553,8 +558,15 @@ class FusedAdamW(FusedAdam):
                 raise RuntimeError("FusedAdamW: max_grad_norm reads every gradient row, set_grad_row_mask says some were not written")
             if len({key[4] for key in buckets}) > 1:
                 raise RuntimeError("FusedAdamW(max_grad_norm): the parameters live on several devices")
-            device, current, stream, n, at, keep = _pack("FusedAdamW", ("gradients",), "p", [t[1] for items in buckets.values() for t in items])
-            self.last_grad_norm, buffer = _norm("FusedAdamW", device, current, stream, n, at, at + 8 * n, at + 16 * n, self.max_grad_norm)
+            items = [t for ts in buckets.values() for t in ts]
+            device, current, stream, n, at, keep = _pack("FusedAdamW", ("gradients",), "p", [t[1] for t in items])
+            rows, rows_keep = None, []
+            if self.capturable:                             # rows that the step leaves alone do not count
+                d = _lib.AdamWDevice()
+                rows_keep = [d]
+                if self._row_form(d, items, items[0][0].device, rows_keep):
+                    rows = ctypes.addressof(d)
+            self.last_grad_norm, buffer = _norm("FusedAdamW", device, current, stream, n, at, at + 8 * n, at + 16 * n, self.max_grad_norm, rows)
             clip = buffer.data_ptr()
         last_of = {key[3:]: key for key in buckets}         # a device counter is advanced by the last launch that reads it
         first, second = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
@@ -591,25 +603,31 @@ class FusedAdamW(FusedAdam):
         keep = [d]
         if self._guard is not None and self._guard[0].device == device:
             d.guard_count, d.guard_limit, d.skipped = self._guard[0].data_ptr(), self._guard[1], self.skipped_steps.data_ptr()
+        self._row_form(d, items, device, keep)
+        return ctypes.addressof(d), keep
+
+    def _row_form(self, d, items, device, keep):
+        """Writes the live rows and row masks that apply to the tensors of `items` into d (its host arrays go to `keep`); -> whether there are any."""
         live = self._live_rows if self._live_rows is not None and self._live_rows.device == device else None
         freeze = self._row_freeze if self._row_freeze is not None and self._row_freeze[0].device == device else None
         rows = self._grad_rows if self._grad_rows is not None and self._grad_rows.device == device else None
-        if live is not None or freeze is not None or rows is not None:
-            params = [t[0] for t in items]
-            if rows is not None and any(p.dim() == 0 or p.shape[0] != rows.numel() for p in params):
-                raise RuntimeError("FusedAdamW.set_grad_row_mask: every parameter must have one row per entry of the mask")
-            width = array.array("i", [p.numel() // p.shape[0] if p.dim() > 0 and p.shape[0] > 0 else 0 for p in params])
-            keep.append(width)
-            d.row_width = _at(width)
-            if live is not None:
-                d.live_rows = live.data_ptr()
-            if rows is not None:
-                d.grad_rows = rows.data_ptr()
-            if freeze is not None:
-                flags = array.array("i", [int(self.param_groups[t[3]].get("name") in freeze[1]) for t in items])
-                if any(fl and p.shape[0] > freeze[0].numel() for fl, p in zip(flags, params)):
-                    raise RuntimeError("FusedAdamW.set_row_freeze: the mask has fewer words than the tensor has rows")
-                if any(flags):
-                    keep.append(flags)
-                    d.row_freeze, d.group_frozen = freeze[0].data_ptr(), _at(flags)
-        return ctypes.addressof(d), keep
+        if live is None and freeze is None and rows is None:
+            return False
+        params = [t[0] for t in items]
+        if rows is not None and any(p.dim() == 0 or p.shape[0] != rows.numel() for p in params):
+            raise RuntimeError("FusedAdamW.set_grad_row_mask: every parameter must have one row per entry of the mask")
+        width = array.array("i", [p.numel() // p.shape[0] if p.dim() > 0 and p.shape[0] > 0 else 0 for p in params])
+        keep.append(width)
+        d.row_width = _at(width)
+        if live is not None:
+            d.live_rows = live.data_ptr()
+        if rows is not None:
+            d.grad_rows = rows.data_ptr()
+        if freeze is not None:
+            flags = array.array("i", [int(self.param_groups[t[3]].get("name") in freeze[1]) for t in items])
+            if any(fl and p.shape[0] > freeze[0].numel() for fl, p in zip(flags, params)):
+                raise RuntimeError("FusedAdamW.set_row_freeze: the mask has fewer words than the tensor has rows")
+            if any(flags):
+                keep.append(flags)
+                d.row_freeze, d.group_frozen = freeze[0].data_ptr(), _at(flags)
+        return True

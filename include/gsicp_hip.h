@@ -456,6 +456,10 @@ int gsicp_adamw_gather_rows(int n, const uint16_t* const* moments, const uint16_
 size_t gsicp_grad_norm_scratch_bytes(int n, const long long* numel, const int* dtype);
 int gsicp_grad_norm(int n, const void* const* grads, const long long* numel, const int* dtype, double max_norm, float* norm_out, float* clip_out, void* scratch,
                     void* stream);
+/* The same without the rows that a step with this device form leaves alone: those behind *live_rows, and the frozen ones of f32 tensors of < 2^32 elements whose group_frozen is
+ * set (row_width, live_rows, row_freeze and group_frozen of *rows are looked at; row_width must be there, grad_rows must not).  What they hold does not matter. */
+int gsicp_grad_norm_rows(int n, const void* const* grads, const long long* numel, const int* dtype, const gsicp_adamw_device* rows, double max_norm, float* norm_out,
+                         float* clip_out, void* scratch, void* stream);
 
 /* Map pruning without reallocation: GaussianModel.prune_points / _prune_optimizer
  * [REF scene/gaussian_model.py:409-447] apply one boolean mask to every parameter, both Adam moments and the per-Gaussian

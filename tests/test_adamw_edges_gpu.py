@@ -1,0 +1,98 @@
+"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _randn(gen, *shape):
+    return torch.randn(shape, device="cuda", generator=gen)
+
+
+# ------------------------------------------------------------------------------------------------ clipping, live rows, frozen rows
+TAILS = [(3,), (1, 3), (15, 3), (1,), (4,), (2,), (7,), (0,), (129,)]
+
+
+@pytest.mark.parametrize("live,bits,freeze", [(None, 32, True)] + [(live, bits, freeze) for live in ("none", "some", "all") for bits, freeze in ((32, True), (32, False), (8, False))])
+@pytest.mark.parametrize("rows,times", [(1, 1), (37, 1), (37, 15), (2777, 1), (300_007, 1)])
+def test_rows_that_are_no_parameters_do_not_count_in_the_norm(rows, times, live, bits, freeze):
+    """Their gradients are NaN: neither the norm nor a row that moves may see them.  Against a twin that has zeros there and no masks."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    gen = torch.Generator(device="cuda").manual_seed(rows + times)
+    tails = [t for t in TAILS if rows < 10_000 or t != (129,)] * times
+    ps = [_randn(gen, rows, *t) for t in tails] + [torch.ones((), device="cuda")]
+    groups = lambda q: [{"params": [p], "name": str(i % len(TAILS)) if p.dim() else "scalar"} for i, p in enumerate(q)]       # noqa: E731
+    a_p, b_p = ([torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2))
+    a, b = (FusedAdamW(groups(q), lr=1e-2, weight_decay=0.1, capturable=True, state_bits=bits, max_grad_norm=0.1, seed=3) for q in (a_p, b_p))
+    n_live = {None: rows, "none": 0, "some": rows * 2 // 3, "all": rows}[live]
+    if live is not None:
+        a.set_live_rows(torch.tensor([n_live], dtype=torch.int32, device="cuda"))
+    frozen = (torch.rand(rows, device="cuda", generator=gen) < 0.4)
+    if freeze:
+        a.set_row_freeze(frozen.to(torch.int32), ("0", "1", "2", "3", "5", "8"))
+    for k in range(3):
+        total, skip = 0.0, []
+        for i, (p, q) in enumerate(zip(a_p, b_p)):
+            g = _randn(gen, *p.shape) * 0.1
+            out = torch.zeros(p.shape[0] if p.dim() else 1, dtype=torch.bool, device="cuda")
+            if p.dim():
+                out[n_live:] = True
+                if freeze and i % len(TAILS) in (0, 1, 2, 3, 5, 8):
+                    out |= frozen
+            skip.append(out)
+            p.grad, q.grad = g.clone(), g.clone()
+            if p.dim():
+                p.grad[out], q.grad[out] = float("nan"), 0.0
+            total += float((q.grad.double() ** 2).sum())
+        before = [p.detach().clone() for p in a_p]
+        a.step()
+        b.step()
+        want = np.sqrt(total)
+        assert abs(float(a.last_grad_norm) - want) <= 2.0 ** -24 * 1.0001 * want, (k, float(a.last_grad_norm), want)      # rounded once
+        assert torch.equal(a.last_grad_norm, b.last_grad_norm)
+        for i, (p, q, out) in enumerate(zip(a_p, b_p, skip)):
+            with torch.no_grad():
+                if p.dim():
+                    assert torch.equal(p[out], before[i][out]), (k, i)
+                    q[out] = before[i][out]                     # the twin decays them
+                assert torch.equal(p, q), (k, i)
+            if p.dim() and bits == 32:
+                for n in ("exp_avg", "exp_avg_sq"):
+                    assert torch.equal(a.state[p][n], b.state[q][n]), (k, i, n)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_clipped_step_follows_the_live_count(bits):
+    """One graph while the live count changes on the device, gradients behind it NaN; replays between eager work, against the host form over the live rows alone."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    rows = 5000
+    shapes = [(rows, 3), (rows, 45), (rows, 1)]
+    p = [torch.nn.Parameter(_randn(gen, *s)) for s in shapes]
+    opt = FusedAdamW(p, lr=1e-2, capturable=True, state_bits=bits, max_grad_norm=0.5)
+    live = torch.tensor([3000], dtype=torch.int32, device="cuda")
+    opt.set_live_rows(live)
+    static = [torch.zeros_like(q) for q in p]
+    for q, g in zip(p, static):
+        q.grad = g
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    norm = opt.last_grad_norm
+    for n in (3000, 1, 5000, 0, 4321):
+        live.fill_(n)
+        new = [_randn(gen, *s) for s in shapes]
+        for g, x in zip(static, new):
+            g.copy_(x)
+            g[n:] = float("nan")
+        before = [q.detach().clone() for q in p]
+        torch.randn(1 << 20, device="cuda").sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = np.sqrt(sum(float((x[:n].double() ** 2).sum()) for x in new))
+        assert abs(float(norm) - want) <= 2.0 ** -24 * 1.0001 * want, n
+        for q, x in zip(p, before):
+            assert bool(torch.isfinite(q).all()) and torch.equal(q[n:], x[n:]) and (n == 0 or not torch.equal(q[:n], x[:n])), n

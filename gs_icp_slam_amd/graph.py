@@ -285,23 +285,8 @@ class MapperIterationGraph:
                 self._iteration()
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
+        self._restore(snap_p, snap_s)
         with torch.no_grad():
-            steps_done = set()
-            for k, v in self.params.items():
-                v.copy_(snap_p[k])
-                st = self.optimizer.state.get(v, {})
-                for name, val in st.items():
-                    if not torch.is_tensor(val):
-                        continue
-                    if name == "step":
-                        if val.data_ptr() in steps_done:
-                            continue
-                        steps_done.add(val.data_ptr())
-                    old = snap_s[v].get(name)
-                    if torch.is_tensor(old):
-                        val.copy_(old)
-                    else:                         # state was created by the warm-up: its pre-warm-up value is zero
-                        val.zero_()
             if skipped0 is not None:
                 self.optimizer.skipped_steps.copy_(skipped0)
         torch.cuda.synchronize(dev)
@@ -333,6 +318,29 @@ class MapperIterationGraph:
         if self.num_rendered is None and hasattr(self.rasterizer, "inner"):
             self.num_rendered = self.rasterizer.inner.num_rendered
         return self
+
+    def _restore(self, snap_p, snap_s):
+        """Parameters and optimiser state as they were before the warm-up.  State that the warm-up created gets its first value: a master weight is its parameter,
+        everything else zero."""
+        with torch.no_grad():
+            steps_done = set()
+            for k, v in self.params.items():
+                v.copy_(snap_p[k])
+                st = self.optimizer.state.get(v, {})
+                for name, val in st.items():
+                    if not torch.is_tensor(val):
+                        continue
+                    if name == "step":
+                        if val.data_ptr() in steps_done:
+                            continue
+                        steps_done.add(val.data_ptr())
+                    old = snap_s[v].get(name)
+                    if torch.is_tensor(old):
+                        val.copy_(old)
+                    elif name == "master":
+                        val.copy_(v)
+                    else:
+                        val.zero_()
 
     def step(self):
         """Replay one iteration (one graph launch).  Returns the static loss tensor (0-dim view; read it when needed)."""

@@ -1,5 +1,8 @@
-"""CPU checks of the AdamW operators at their edges: refusals of the row-aware gradient norm."""
+"""CPU checks of the AdamW operators at their edges: refusals of the row-aware gradient norm, optimiser state around a capture."""
 import ctypes
+
+import pytest
+import torch
 
 
 def _one(*x):
@@ -25,3 +28,36 @@ def test_norm_without_rows_that_are_left_alone_refuses_before_it_launches():
     assert norm(D(**ok), grad=0) == -2 and norm(D(**ok), grad=1 << 58) == -2 and norm(D(**ok), out=None) == -2 and norm(D(**ok), n=-1) == -2
     assert norm(D(**ok), numel=1 << 30, scratch=None) == -2
     assert b"gsicp_grad_norm" in lib.gsicp_last_error()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_made_by_the_warm_up_of_a_capture_gets_its_first_value(bits):
+    """Parameters and state as a capture's warm-up leaves them, put back: a master weight that it made is the parameter, not zero."""
+    from gs_icp_slam_amd.graph import MapperIterationGraph
+    from gs_icp_slam_amd.optim import FusedAdamW
+    params = {k: torch.nn.Parameter(torch.full((300,), v, dtype=dt)) for k, v, dt in (("a", 1.5, torch.bfloat16), ("b", -2.0, torch.float16), ("c", 3.0, torch.float32),
+                                                                                    ("old", 0.25, torch.bfloat16))}
+    mg = MapperIterationGraph.__new__(MapperIterationGraph)
+    mg.params, mg.optimizer = params, FusedAdamW(params.values(), state_bits=bits, master_weights=True, capturable=True)
+    mg.optimizer._new_state(params["old"], torch.zeros((), dtype=torch.int32) + 4)
+    mg.optimizer.state[params["old"]]["master"].fill_(0.250001)
+    snap_p = {k: p.detach().clone() for k, p in params.items()}
+    snap_s = {p: {k: v.clone() for k, v in mg.optimizer.state.get(p, {}).items()} for p in params.values()}
+    shared = torch.zeros((), dtype=torch.int32)
+    with torch.no_grad():
+        for k, p in params.items():
+            if k != "old":
+                mg.optimizer._new_state(p, shared)
+            p.add_(1.0)
+            for v in mg.optimizer.state[p].values():
+                v.add_(1)
+    mg._restore(snap_p, snap_s)
+    for k, p in params.items():
+        st = mg.optimizer.state[p]
+        assert torch.equal(p, snap_p[k]) and int(st["step"]) == (4 if k == "old" else 0)
+        assert ("master" in st) == (p.dtype != torch.float32)
+        if k == "old":
+            assert torch.equal(st["master"], torch.full((300,), 0.250001))
+        elif k != "c":
+            assert torch.equal(st["master"], p.detach().float())
+        assert all(not bool(st[n].any()) for n in (("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps")))

@@ -1,7 +1,10 @@
-"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters."""
+"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture."""
 import numpy as np
 import pytest
 import torch
+
+from gs_icp_slam_amd import synth
+from tests.util import make_settings, torch_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +99,55 @@ def test_a_captured_clipped_step_follows_the_live_count(bits):
         assert abs(float(norm) - want) <= 2.0 ** -24 * 1.0001 * want, n
         for q, x in zip(p, before):
             assert bool(torch.isfinite(q).all()) and torch.equal(q[n:], x[n:]) and (n == 0 or not torch.equal(q[:n], x[:n])), n
+
+
+# ------------------------------------------------------------------------------------------------ the captured mapper iteration
+def _mapper(P, W, H):
+    """-> (raw parameters of a map in f32, view settings, colour and depth images of a map that differs from it)."""
+    from diff_gaussian_rasterization import GaussianRasterizer
+    cfg = dict(synth.REPLICA)
+    cam = synth.make_camera(W, H, cfg["fx"] * W / cfg["W"], cfg["fy"] * H / cfg["H"], synth.DEFAULT_POSE_A)
+    g = synth.s_map(P, seed=5)
+    raw = {"means3D": torch.from_numpy(g["means3D"]), "scales": torch.log(torch.from_numpy(g["scales"])), "rotations": torch.from_numpy(g["rotations"]),
+           "opacities": torch.logit(torch.from_numpy(g["opacities"]).clamp(1e-4, 1 - 1e-4)), "shs": torch.from_numpy(g["shs"])}
+    rs = make_settings(cam, [0.0, 0.0, 0.0])
+    t2 = torch_inputs(synth.s_map(P, seed=5, perturb_seed=7))
+    with torch.no_grad():
+        depth, color, _, _ = GaussianRasterizer(rs)(means3D=t2["means3D"], means2D=torch.zeros_like(t2["means3D"]), shs=t2["shs"], opacities=t2["opacities"],
+                                                    scales=t2["scales"], rotations=t2["rotations"])
+    return raw, cam, rs, color, depth
+
+
+MAPPER_LRS = {"means3D": 4e-6, "shs": 2.5e-3, "opacities": 0.05, "scales": 5e-3, "rotations": 1e-3}
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_masters_that_a_capture_makes_start_at_their_parameters(bits):
+    """16-bit parameters with masters and no step before the capture, dense gradients because of the clipping."""
+    from gs_icp_slam_amd.graph import MapperIterationGraph
+    from gs_icp_slam_amd.optim import FusedAdamW
+    W, H = 320, 200
+    raw, cam, rs, color, depth = _mapper(20000, W, H)
+    half = ("shs", "opacities")
+    params = {k: v.cuda().to(torch.bfloat16 if k in half else torch.float32).contiguous().requires_grad_(True) for k, v in raw.items()}
+    opt = FusedAdamW([{"params": [params[k]], "lr": lr} for k, lr in MAPPER_LRS.items()], lr=0.0, eps=1e-15, weight_decay=0.0, capturable=True, state_bits=bits,
+                     master_weights=True, max_grad_norm=1e-3)
+    mg = MapperIterationGraph(params, opt, H, W, cam["tanfovx"], cam["tanfovy"], sh_degree=0, capacity=2_000_000, warmup=2)
+    mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+    start = {k: p.detach().clone() for k, p in params.items()}
+    mg.capture()
+    for k, p in params.items():
+        assert torch.equal(p, start[k])
+        assert k not in half or torch.equal(opt.state[p]["master"], start[k].float())
+    for n in (1, 2, 3):
+        mg.set_view(rs.viewmatrix, rs.projmatrix, rs.campos, color, depth)
+        assert np.isfinite(float(mg.step()))
+        torch.cuda.synchronize()
+    assert int(opt.state[params["means3D"]]["step"]) == 3
+    for k in half:
+        p, w = params[k].detach(), opt.state[params[k]]["master"]
+        assert torch.equal(w.bfloat16(), p) and not torch.equal(w, start[k].float())
+        # step t moves an element by at most lr sqrt(t) with exact moments (Cauchy-Schwarz over the weights of m and v); 8-bit codes are within an eighth of the moments
+        # and an element at their floors moves by at most three times its block's largest step: 4 lr sqrt(t) holds for both
+        assert (w - start[k].float()).abs().max() <= MAPPER_LRS[k] * (1 + 2 ** 0.5 + 3 ** 0.5) * 4, k
+    mg.release()

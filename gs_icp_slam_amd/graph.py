@@ -321,7 +321,7 @@ class MapperIterationGraph:
 
     def _restore(self, snap_p, snap_s):
         """Parameters and optimiser state as they were before the warm-up.  State that the warm-up created gets its first value: a master weight is its parameter,
-        everything else zero."""
+        everything else zero; a step count that it took from the host to the device keeps its value."""
         with torch.no_grad():
             steps_done = set()
             for k, v in self.params.items():
@@ -337,6 +337,8 @@ class MapperIterationGraph:
                     old = snap_s[v].get(name)
                     if torch.is_tensor(old):
                         val.copy_(old)
+                    elif old is not None:         # a step count that the host kept
+                        val.fill_(old)
                     elif name == "master":
                         val.copy_(v)
                     else:

@@ -61,3 +61,26 @@ def test_state_made_by_the_warm_up_of_a_capture_gets_its_first_value(bits):
         elif k != "c":
             assert torch.equal(st["master"], p.detach().float())
         assert all(not bool(st[n].any()) for n in (("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps")))
+
+
+@pytest.mark.parametrize("counts", [(7, 7, 0), (3, 5, 3)])
+@pytest.mark.parametrize("adamw", [True, False])
+def test_a_step_count_of_the_host_survives_a_capture(adamw, counts):
+    """A state with host step counts (made without capturable, or by hand) goes to the device in the warm-up; putting it back must not lose the count."""
+    from gs_icp_slam_amd.graph import MapperIterationGraph
+    from gs_icp_slam_amd.optim import FusedAdam, FusedAdamW
+    params = {k: torch.nn.Parameter(torch.ones(300)) for k in "abc"}
+    mg = MapperIterationGraph.__new__(MapperIterationGraph)
+    mg.params, mg.optimizer = params, (FusedAdamW if adamw else FusedAdam)(params.values(), capturable=True)
+    for p, n in zip(params.values(), counts):
+        mg.optimizer.state[p].update(step=n, exp_avg=torch.full((300,), 0.5), exp_avg_sq=torch.full((300,), 0.25))
+    snap_p = {k: p.detach().clone() for k, p in params.items()}
+    snap_s = {p: {k: v.clone() if torch.is_tensor(v) else v for k, v in mg.optimizer.state[p].items()} for p in params.values()}
+    device_counts = {}
+    for p, n in zip(params.values(), counts):
+        step = device_counts.setdefault(n, torch.full((), n + 2, dtype=torch.int32))      # as two warm-up iterations leave it, shared by equal counts
+        mg.optimizer.state[p].update(step=step, exp_avg=torch.full((300,), 9.0), exp_avg_sq=torch.full((300,), 9.0))
+    mg._restore(snap_p, snap_s)
+    for p, n in zip(params.values(), counts):
+        st = mg.optimizer.state[p]
+        assert int(st["step"]) == n and bool((st["exp_avg"] == 0.5).all()) and bool((st["exp_avg_sq"] == 0.25).all())

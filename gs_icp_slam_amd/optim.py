@@ -486,7 +486,7 @@ class FusedAdamW(FusedAdam):
 
     def load_state_dict(self, state_dict):
         """torch's load casts every state tensor to its parameter's dtype; moments, masters and 8-bit codes keep their own here, and parameters that shared a step counter
-        share it again."""
+        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
         for i in saved:
@@ -505,6 +505,12 @@ class FusedAdamW(FusedAdam):
                 elif torch.is_tensor(v):
                     v = v.detach().to(device=p.device, copy=True)
                 self.state[p][k] = v
+            st = self.state.get(p)
+            if st:
+                if not self.master_weights or p.dtype == torch.float32:
+                    st.pop("master", None)
+                elif "master" not in st:
+                    st["master"] = p.detach().float()
 
     def _new_state(self, p, step):
         st = self.state[p]

@@ -84,3 +84,32 @@ def test_a_step_count_of_the_host_survives_a_capture(adamw, counts):
     for p, n in zip(params.values(), counts):
         st = mg.optimizer.state[p]
         assert int(st["step"]) == n and bool((st["exp_avg"] == 0.5).all()) and bool((st["exp_avg_sq"] == 0.25).all())
+
+
+# ------------------------------------------------------------------------------------------------ state dicts of other optimisers
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("saved,loaded", [(True, True), (True, False), (False, True), (False, False)])
+def test_masters_after_loading_are_those_that_the_optimiser_keeps(bits, saved, loaded):
+    from gs_icp_slam_amd.optim import FusedAdamW
+    dtypes = [torch.bfloat16, torch.float16, torch.float32, torch.bfloat16]
+    ps = [torch.nn.Parameter(torch.randn(130).to(dt)) for dt in dtypes]
+    a = FusedAdamW(ps, state_bits=bits, master_weights=saved)
+    for p in ps[:3]:
+        a._new_state(p, 4)
+        if "master" in a.state[p]:
+            a.state[p]["master"] += 1e-4
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    b = FusedAdamW(qs, state_bits=bits, master_weights=loaded)
+    b.load_state_dict(a.state_dict())
+    for p, q in zip(ps[:3], qs):
+        st = b.state[q]
+        assert ("master" in st) == (loaded and q.dtype != torch.float32)
+        if "master" in st:
+            assert st["master"].dtype == torch.float32 and torch.equal(st["master"], a.state[p]["master"] if saved else q.detach().float())
+            assert st["master"].data_ptr() != q.data_ptr()
+    assert not b.state.get(qs[3])                            # not stepped yet: the first step makes its state
+    # masters of 16-bit parameters do not belong to the f32 parameters that take over their state
+    wide = [torch.nn.Parameter(p.detach().float()) for p in ps]
+    c = FusedAdamW(wide, state_bits=bits, master_weights=True)
+    c.load_state_dict(a.state_dict())
+    assert all("master" not in c.state[q] for q in wide[:3])

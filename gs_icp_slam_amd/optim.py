@@ -486,13 +486,16 @@ class FusedAdamW(FusedAdam):
 
     def load_state_dict(self, state_dict):
         """torch's load casts every state tensor to its parameter's dtype; moments, masters and 8-bit codes keep their own here, and parameters that shared a step counter
-        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped."""
+        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped.  A state of FusedAdam, which has no weight decay, leaves that of each group as it is here."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
         for i in saved:
             if any(k not in state_dict["state"].get(i, dict.fromkeys(names)) for k in names):
                 raise ValueError(f"FusedAdamW(state_bits={self.state_bits}): the state was saved with another width of the moments")
+        decays = [g["weight_decay"] for g in self.param_groups]
         super().load_state_dict(state_dict)
+        for g, decay in zip(self.param_groups, decays):     # FusedAdam's groups have none
+            g.setdefault("weight_decay", decay)
         steps = {}
         for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
             for k, v in state_dict["state"].get(i, {}).items():

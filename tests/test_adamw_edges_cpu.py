@@ -113,3 +113,19 @@ def test_masters_after_loading_are_those_that_the_optimiser_keeps(bits, saved, l
     c = FusedAdamW(wide, state_bits=bits, master_weights=True)
     c.load_state_dict(a.state_dict())
     assert all("master" not in c.state[q] for q in wide[:3])
+
+
+def test_a_state_without_weight_decay_leaves_that_of_the_groups():
+    from gs_icp_slam_amd.optim import FusedAdam, FusedAdamW
+    make = lambda: [{"params": [torch.nn.Parameter(torch.ones(9))]}, {"params": [torch.nn.Parameter(torch.ones(5))], "lr": 0.25}]       # noqa: E731
+    a = FusedAdam(make(), lr=0.5)
+    for g in a.param_groups:
+        a.state[g["params"][0]].update(step=3, exp_avg=torch.ones_like(g["params"][0]), exp_avg_sq=torch.ones_like(g["params"][0]))
+    groups = make()
+    groups[1]["weight_decay"] = 0.3
+    b = FusedAdamW(groups, lr=1.0, weight_decay=0.05)
+    b.load_state_dict(a.state_dict())
+    assert [g["weight_decay"] for g in b.param_groups] == [0.05, 0.3] and [g["lr"] for g in b.param_groups] == [0.5, 0.25]
+    c = FusedAdamW(make(), weight_decay=0.7)
+    c.load_state_dict(b.state_dict())
+    assert [g["weight_decay"] for g in c.param_groups] == [0.05, 0.3]              # a state that has it says it

@@ -486,12 +486,17 @@ class FusedAdamW(FusedAdam):
 
     def load_state_dict(self, state_dict):
         """torch's load casts every state tensor to its parameter's dtype; moments, masters and 8-bit codes keep their own here, and parameters that shared a step counter
-        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped.  A state of FusedAdam, which has no weight decay, leaves that of each group as it is here."""
+        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped.  A state of FusedAdam, which has no weight decay, leaves that of each group as it is here.  States of torch.optim.Adam and
+        AdamW are taken, but not with amsgrad, maximize or a weight decay that is added to the gradient."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
         for i in saved:
             if any(k not in state_dict["state"].get(i, dict.fromkeys(names)) for k in names):
                 raise ValueError(f"FusedAdamW(state_bits={self.state_bits}): the state was saved with another width of the moments")
+        for g in state_dict["param_groups"]:
+            for k, wanted in (("amsgrad", False), ("maximize", False), ("decoupled_weight_decay", True)):
+                if bool(g.get(k, wanted)) != wanted and (k != "decoupled_weight_decay" or g.get("weight_decay", 0) != 0):
+                    raise ValueError(f"FusedAdamW: the state was saved with {k}={g[k]}")
         decays = [g["weight_decay"] for g in self.param_groups]
         super().load_state_dict(state_dict)
         for g, decay in zip(self.param_groups, decays):     # FusedAdam's groups have none

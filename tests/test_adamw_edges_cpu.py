@@ -129,3 +129,23 @@ def test_a_state_without_weight_decay_leaves_that_of_the_groups():
     c = FusedAdamW(make(), weight_decay=0.7)
     c.load_state_dict(b.state_dict())
     assert [g["weight_decay"] for g in c.param_groups] == [0.05, 0.3]              # a state that has it says it
+
+
+@pytest.mark.parametrize("cls,kw,taken", [("AdamW", {}, True), ("AdamW", dict(weight_decay=0.3), True), ("Adam", {}, True), ("Adam", dict(weight_decay=0.1), False),
+                                          ("AdamW", dict(amsgrad=True), False), ("AdamW", dict(maximize=True), False), ("Adam", dict(maximize=True), False)])
+def test_states_of_torch_optimisers_with_another_update_are_refused(cls, kw, taken):
+    from gs_icp_slam_amd.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.ones(9))
+    a = getattr(torch.optim, cls)([p], lr=0.125, **kw)
+    p.grad = torch.ones(9)
+    a.step()
+    opt = FusedAdamW([torch.nn.Parameter(torch.ones(9))])
+    if taken:
+        opt.load_state_dict(a.state_dict())
+        st = opt.state[opt.param_groups[0]["params"][0]]
+        assert st["step"] == 1 and isinstance(st["step"], int) and torch.equal(st["exp_avg"], a.state[p]["exp_avg"])
+        assert opt.param_groups[0]["lr"] == 0.125 and opt.param_groups[0]["weight_decay"] == a.param_groups[0]["weight_decay"]
+    else:
+        with pytest.raises(ValueError, match="FusedAdamW"):
+            opt.load_state_dict(a.state_dict())
+        assert not opt.state and opt.param_groups[0]["lr"] == 1e-3

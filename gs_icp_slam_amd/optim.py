@@ -486,7 +486,7 @@ class FusedAdamW(FusedAdam):
 
     def load_state_dict(self, state_dict):
         """torch's load casts every state tensor to its parameter's dtype; moments, masters and 8-bit codes keep their own here, and parameters that shared a step counter
-        share it again.  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped.  A state of FusedAdam, which has no weight decay, leaves that of each group as it is here.  States of torch.optim.Adam and
+        share it again (those of torch's optimisers, which count per parameter, share one where they agree).  Masters are kept as this optimiser has them: those that the state lacks are made from the parameters (load these first), others are dropped.  A state of FusedAdam, which has no weight decay, leaves that of each group as it is here.  States of torch.optim.Adam and
         AdamW are taken, but not with amsgrad, maximize or a weight decay that is added to the gradient."""
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("moments", "block_exps")
@@ -505,7 +505,7 @@ class FusedAdamW(FusedAdam):
         for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
             for k, v in state_dict["state"].get(i, {}).items():
                 if k == "step":
-                    key = (v.data_ptr() if torch.is_tensor(v) else int(v), p.device)
+                    key = (v.data_ptr() if torch.is_tensor(v) and v.dtype == torch.int32 else int(v), p.device)      # torch's optimisers: a counter per parameter
                     if self.capturable:
                         v = steps.setdefault(key, torch.full((), int(v), dtype=torch.int32, device=p.device))
                     else:

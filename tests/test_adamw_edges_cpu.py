@@ -149,3 +149,29 @@ def test_states_of_torch_optimisers_with_another_update_are_refused(cls, kw, tak
         with pytest.raises(ValueError, match="FusedAdamW"):
             opt.load_state_dict(a.state_dict())
         assert not opt.state and opt.param_groups[0]["lr"] == 1e-3
+
+
+def test_counts_of_a_torch_optimiser_that_agree_share_one_device_counter():
+    """One counter per parameter would mean a launch per parameter, and no shared counter for the captured iteration to advance."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    ps = [torch.nn.Parameter(torch.ones(n)) for n in (5, 6, 7, 8)]
+    a = torch.optim.AdamW(ps)
+    for k in range(3):
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        if k == 1:
+            ps[3].grad = None
+        a.step()
+    opt = FusedAdamW([torch.nn.Parameter(p.detach().clone()) for p in ps], capturable=True)
+    opt.load_state_dict(a.state_dict())
+    counters = [opt.state[p]["step"] for p in opt.param_groups[0]["params"]]
+    assert [int(c) for c in counters] == [3, 3, 3, 2] and all(c.dtype == torch.int32 and c.shape == () for c in counters)
+    assert len({c.data_ptr() for c in counters[:3]}) == 1 and counters[3].data_ptr() != counters[0].data_ptr()
+    # counters of one's own that agree by chance stay apart: they need not agree after the next step
+    b = FusedAdamW([torch.nn.Parameter(p.detach().clone()) for p in ps], capturable=True)
+    own = [torch.full((), 4, dtype=torch.int32) for _ in range(2)]
+    for p, c in zip(b.param_groups[0]["params"], (own[0], own[0], own[1], own[1])):
+        b._new_state(p, c)
+    opt.load_state_dict(b.state_dict())
+    counters = [opt.state[p]["step"].data_ptr() for p in opt.param_groups[0]["params"]]
+    assert counters[0] == counters[1] != counters[2] == counters[3]

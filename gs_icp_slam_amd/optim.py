@@ -191,7 +191,7 @@ class FusedAdam(torch.optim.Optimizer):
                 if freeze is not None:
                     flags = [1 if self.param_groups[t[6][0]].get("name") in freeze[1] else 0 for t in items]
                     for t, fl in zip(items, flags):
-                        if fl and t[0].shape[0] > freeze[0].numel():
+                        if fl and t[0].dim() > 0 and t[0].shape[0] > freeze[0].numel():
                             raise RuntimeError("FusedAdam.set_row_freeze: the mask has fewer words than the tensor has rows")
                     if any(flags):
                         freeze_ptr, FR = ctypes.c_void_p(freeze[0].data_ptr()), (ctypes.c_int * n)(*flags)
@@ -639,7 +639,7 @@ class FusedAdamW(FusedAdam):
             d.grad_rows = rows.data_ptr()
         if freeze is not None:
             flags = array.array("i", [int(self.param_groups[t[3]].get("name") in freeze[1]) for t in items])
-            if any(fl and p.shape[0] > freeze[0].numel() for fl, p in zip(flags, params)):
+            if any(fl and p.dim() > 0 and p.shape[0] > freeze[0].numel() for fl, p in zip(flags, params)):
                 raise RuntimeError("FusedAdamW.set_row_freeze: the mask has fewer words than the tensor has rows")
             if any(flags):
                 keep.append(flags)

@@ -101,6 +101,23 @@ def test_a_captured_clipped_step_follows_the_live_count(bits):
             assert bool(torch.isfinite(q).all()) and torch.equal(q[n:], x[n:]) and (n == 0 or not torch.equal(q[:n], x[:n])), n
 
 
+@pytest.mark.parametrize("adamw", [True, False])
+def test_a_parameter_without_rows_in_a_frozen_group(adamw):
+    """A 0-dim parameter has no row to freeze: it moves, the frozen rows beside it do not."""
+    from gs_icp_slam_amd.optim import FusedAdam, FusedAdamW
+    p, scalar = torch.nn.Parameter(torch.ones(6, 2, device="cuda")), torch.nn.Parameter(torch.ones((), device="cuda"))
+    opt = (FusedAdamW if adamw else FusedAdam)([{"params": [p, scalar], "name": "xyz"}], lr=0.1, capturable=True)
+    frozen = torch.tensor([1, 0, 0, 1, 0, 1], dtype=torch.int32, device="cuda")
+    opt.set_row_freeze(frozen, ("xyz",))
+    p.grad, scalar.grad = torch.ones_like(p), torch.ones_like(scalar)
+    opt.step()
+    moved = (p != 1).all(1)
+    assert moved.tolist() == (frozen == 0).tolist() and float(scalar) < 1.0
+    with pytest.raises(RuntimeError):
+        opt.set_row_freeze(frozen[:5].clone(), ("xyz",))
+        opt.step()
+
+
 # ------------------------------------------------------------------------------------------------ the captured mapper iteration
 def _mapper(P, W, H):
     """-> (raw parameters of a map in f32, view settings, colour and depth images of a map that differs from it)."""

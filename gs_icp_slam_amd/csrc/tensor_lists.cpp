@@ -82,6 +82,7 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 const at::ScalarType dt = t.scalar_type();
                 if (!t.is_cuda()) { why = "must live on the HIP device (gfx950): there is no CPU path"; break; }
                 if (t.layout() != at::kStrided || !t.is_contiguous()) { why = "must be contiguous"; break; }
+                if (t.is_neg()) { why = "must not be negated lazily (resolve_neg())"; break; }      // the memory holds the other sign
                 if (device < 0) device = t.get_device();
                 if (t.get_device() != device) { why = "must live on one device"; break; }
                 if (l == 0) {

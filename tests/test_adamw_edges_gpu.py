@@ -1,4 +1,4 @@
-"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture."""
+"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture; lists."""
 import numpy as np
 import pytest
 import torch
@@ -112,7 +112,7 @@ def test_a_parameter_without_rows_in_a_frozen_group(adamw):
     p.grad, scalar.grad = torch.ones_like(p), torch.ones_like(scalar)
     opt.step()
     moved = (p != 1).all(1)
-    assert moved.tolist() == (frozen == 0).tolist() and float(scalar) < 1.0
+    assert moved.tolist() == (frozen == 0).tolist() and float(scalar.detach()) < 1.0
     with pytest.raises(RuntimeError):
         opt.set_row_freeze(frozen[:5].clone(), ("xyz",))
         opt.step()
@@ -168,3 +168,25 @@ def test_masters_that_a_capture_makes_start_at_their_parameters(bits):
         # and an element at their floors moves by at most three times its block's largest step: 4 lr sqrt(t) holds for both
         assert (w - start[k].float()).abs().max() <= MAPPER_LRS[k] * (1 + 2 ** 0.5 + 3 ** 0.5) * 4, k
     mg.release()
+
+
+# ------------------------------------------------------------------------------------------------ lists of tensors
+def test_tensors_that_are_negated_lazily_are_refused():
+    """The imaginary part of a conjugate holds the other sign in memory."""
+    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step, grad_norm
+    g = torch.conj(torch.tensor([1 + 2j], device="cuda")).imag
+    assert g.is_neg() and g.is_contiguous() and float(g) == -2.0
+    new = lambda: torch.zeros(1, device="cuda")              # noqa: E731
+    p, m, v = new(), new(), new()
+    for lists in (([p], [g], [m], [v]), ([g], [p], [m], [v]), ([p], [m], [g], [v])):
+        with pytest.raises(RuntimeError, match="negated"):
+            adamw_step(*lists, lr=0.1, step=1)
+    q = torch.nn.Parameter(new())
+    q.grad = g
+    with pytest.raises(RuntimeError, match="negated"):
+        FusedAdamW([q]).step()
+    with pytest.raises(RuntimeError, match="negated"):
+        grad_norm([g])
+    assert float(p) == float(m) == float(v) == 0.0
+    adamw_step([p], [g.resolve_neg()], [m], [v], lr=0.1, step=1)
+    assert float(m) < 0 < float(p)

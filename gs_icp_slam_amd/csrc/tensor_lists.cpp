@@ -3,6 +3,7 @@
 // ~0.2 us together) cost more than the kernel; here they are a few loads.
 //
 //   pack(what, names, rules, list, ...) -> (device index, whether it is the current one, its current stream, n, address, keep)
+//   wrote(keep, which)                  after a launch: raises the version counters of the tensors that it writes
 //
 // One rule (a character) and one name (for the errors) per list; the first list has rule 'p' or 'c' and says device, length and element counts:
 //   p  float32 / bfloat16 / float16 (their codes are recorded)      g  the first list's dtype, read only      f  float32         h  int16
@@ -118,7 +119,33 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+// The tensors of the lists whose bit is set in `which` were written: autograd must notice when a backward meets one that it saved before.
+PyObject* wrote(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    const long which = nargs == 2 && PyTuple_Check(args[0]) ? PyLong_AsLong(args[1]) : -1;
+    if (which < 0) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "wrote(keep, which)");
+        return nullptr;
+    }
+    try {
+        for (Py_ssize_t l = 0; l + 1 < PyTuple_GET_SIZE(args[0]); ++l) {
+            PyObject* seq = PyTuple_GET_ITEM(args[0], l + 1);
+            if (!(which >> l & 1) || !(PyList_Check(seq) || PyTuple_Check(seq))) continue;
+            for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
+                PyObject* item = PySequence_Fast_GET_ITEM(seq, i);
+                if (!THPVariable_Check(item)) continue;
+                const at::Tensor& t = THPVariable_Unpack(item);
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            }
+        }
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+    Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {{"pack", (PyCFunction)(void (*)(void))pack, METH_FASTCALL, "pack(what, names, rules, list, ...) -> (device index, current, stream, n, address, keep)"},
+                         {"wrote", (PyCFunction)(void (*)(void))wrote, METH_FASTCALL, "wrote(keep, which): raises the version counters of the lists whose bit is set in which"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", "lists of torch tensors as host arrays of the C ABI", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -357,6 +357,7 @@ def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, 
         _call("gsicp_adamw_step", device, current, *args, clip, dev, stream)
     else:
         _call("gsicp_adamw_step_8bit", device, current, *args, int(seed) & 0xFFFFFFFF, _at(place), clip, dev, stream)
+    _tensor_lists.wrote(keep, 0b10001)        # parameters and masters: a backward may have saved them (no graph reaches the moments; each list of 64 costs 0.8 us)
     return norm
 
 

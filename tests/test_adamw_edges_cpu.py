@@ -175,3 +175,20 @@ def test_counts_of_a_torch_optimiser_that_agree_share_one_device_counter():
     opt.load_state_dict(b.state_dict())
     counters = [opt.state[p]["step"].data_ptr() for p in opt.param_groups[0]["params"]]
     assert counters[0] == counters[1] != counters[2] == counters[3]
+
+
+# ------------------------------------------------------------------------------------------------ lists of tensors
+def test_written_lists_raise_their_version_counters():
+    from gs_icp_slam_amd import _tensor_lists
+    a, b, c = [torch.zeros(2), torch.zeros(0)], (torch.zeros(3),), [None, torch.zeros(1)]
+    version = lambda: [t._version for t in (*a, *b, c[1])]           # noqa: E731
+    _tensor_lists.wrote((b"", a, b, c), 0b101)
+    assert version() == [1, 1, 0, 1]
+    _tensor_lists.wrote((b"", a, b, c), 0b010)
+    assert version() == [1, 1, 1, 1]
+    with torch.inference_mode():
+        still = torch.zeros(2)                                       # counts no versions
+    _tensor_lists.wrote((b"", [still]), 1)
+    for args in ((), ((b"", a),), ((b"", a), -1), ([b"", a], 1), ((b"", a), "x")):
+        with pytest.raises(TypeError):
+            _tensor_lists.wrote(*args)

@@ -1,4 +1,4 @@
-"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture; lists."""
+"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture; lists; autograd."""
 import numpy as np
 import pytest
 import torch
@@ -190,3 +190,36 @@ def test_tensors_that_are_negated_lazily_are_refused():
     assert float(p) == float(m) == float(v) == 0.0
     adamw_step([p], [g.resolve_neg()], [m], [v], lr=0.1, step=1)
     assert float(m) < 0 < float(p)
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+@pytest.mark.parametrize("which", ["adamw_step", "adamw_step_8bit", "FusedAdamW", "FusedAdamW capturable", "FusedAdamW masters"])
+def test_a_backward_over_what_a_step_has_written_is_refused(which):
+    """As after torch's optimisers: the product saved the parameter, the step changed it."""
+    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step, adamw_step_8bit, new_moments_8bit
+    dtype = torch.bfloat16 if "masters" in which else torch.float32
+    p = torch.nn.Parameter(torch.ones(9, device="cuda", dtype=dtype))
+    other = torch.nn.Parameter(torch.ones(9, device="cuda", dtype=dtype))
+    p.grad = torch.ones_like(p)
+    loss = (p * other).sum()
+    version = p.grad._version
+    if which == "adamw_step":
+        adamw_step([p], [p.grad], [torch.zeros_like(p)], [torch.zeros_like(p)], lr=0.1, step=1)
+    elif which == "adamw_step_8bit":
+        m, x = new_moments_8bit(p)
+        adamw_step_8bit([p], [p.grad], [m], [x], lr=0.1, step=1)
+    else:
+        FusedAdamW([p], capturable="capturable" in which, master_weights="masters" in which).step()
+    assert p.grad._version == version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    (p * other).sum().backward()                                     # of the new values
+
+
+def test_a_step_over_inference_tensors():
+    from gs_icp_slam_amd.optim import adamw_step
+    with torch.inference_mode():
+        lists = [[torch.full((5,), x, device="cuda")] for x in (1.0, 1.0, 0.0, 0.0)]
+        adamw_step(*lists, lr=0.1, step=1)
+    adamw_step(*lists, lr=0.1, step=2)
+    assert bool((lists[0][0] < 0.9).all())

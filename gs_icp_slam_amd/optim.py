@@ -200,6 +200,7 @@ class FusedAdam(torch.optim.Optimizer):
                                                       ctypes.c_void_p(items[0][5].data_ptr()), bump, guard_ptr, guard_lim,
                                                       skip_ptr, live_ptr, RW, freeze_ptr, FR, ctypes.c_void_p(rows.data_ptr()) if rows is not None else None,
                                                       stream), "gsicp_adam_step_sparse")
+            _native_lists().wrote((None, [t[0] for t in items]), 1)      # autograd must notice when a backward meets one that it saved before
         # Device lr arrays are NEVER freed: a captured MapperIterationGraph holds their addresses, and an eager step() that happens
         # to see fewer gradients (zero_grad(set_to_none=True), different chunking) must not hand that memory back to the caching allocator
         # while a graph may still replay.  One entry is <= 8 doubles; the number of distinct buckets an optimiser ever sees is a handful.
@@ -251,6 +252,7 @@ class FusedAdam(torch.optim.Optimizer):
                     N = (ctypes.c_longlong * n)(*[t[0].numel() for t in chunk])
                     LR = (ctypes.c_float * n)(*[t[4] for t in chunk])
                     _lib.check(lib.gsicp_adam_step(n, P, G, M, V, N, LR, b1, b2, eps, step, stream), "gsicp_adam_step")
+            _native_lists().wrote((None, [t[0] for t in items]), 1)
         return loss
 
 
@@ -259,9 +261,7 @@ _BLOCK = 128                       # elements per base exponent of 8-bit moments
 _tensor_lists = None
 
 
-def _pack(what, names, rules, *lists):
-    """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, whether it is the current one, its current stream, n, address of the arrays, what
-    keeps them and the tensors alive).  The arrays: n addresses per list, n element counts (8 bytes each), n dtype codes."""
+def _native_lists():
     global _tensor_lists
     if _tensor_lists is None:
         try:
@@ -269,7 +269,13 @@ def _pack(what, names, rules, *lists):
         except ImportError as e:
             raise ImportError("gs_icp_slam_amd/_tensor_lists not found: build it with `python -m gs_icp_slam_amd.build`") from e
         _tensor_lists = module
-    return _tensor_lists.pack(what, names, rules, *lists)
+    return _tensor_lists
+
+
+def _pack(what, names, rules, *lists):
+    """Lists of tensors, checked, as host arrays (csrc/tensor_lists.cpp) -> (device index, whether it is the current one, its current stream, n, address of the arrays, what
+    keeps them and the tensors alive).  The arrays: n addresses per list, n element counts (8 bytes each), n dtype codes."""
+    return _native_lists().pack(what, names, rules, *lists)
 
 
 def _at(a):

@@ -193,10 +193,10 @@ def test_tensors_that_are_negated_lazily_are_refused():
 
 
 # ------------------------------------------------------------------------------------------------ autograd
-@pytest.mark.parametrize("which", ["adamw_step", "adamw_step_8bit", "FusedAdamW", "FusedAdamW capturable", "FusedAdamW masters"])
+@pytest.mark.parametrize("which", ["adamw_step", "adamw_step_8bit", "FusedAdamW", "FusedAdamW capturable", "FusedAdamW masters", "FusedAdam", "FusedAdam capturable"])
 def test_a_backward_over_what_a_step_has_written_is_refused(which):
     """As after torch's optimisers: the product saved the parameter, the step changed it."""
-    from gs_icp_slam_amd.optim import FusedAdamW, adamw_step, adamw_step_8bit, new_moments_8bit
+    from gs_icp_slam_amd.optim import FusedAdam, FusedAdamW, adamw_step, adamw_step_8bit, new_moments_8bit
     dtype = torch.bfloat16 if "masters" in which else torch.float32
     p = torch.nn.Parameter(torch.ones(9, device="cuda", dtype=dtype))
     other = torch.nn.Parameter(torch.ones(9, device="cuda", dtype=dtype))
@@ -208,8 +208,10 @@ def test_a_backward_over_what_a_step_has_written_is_refused(which):
     elif which == "adamw_step_8bit":
         m, x = new_moments_8bit(p)
         adamw_step_8bit([p], [p.grad], [m], [x], lr=0.1, step=1)
-    else:
+    elif "AdamW" in which:
         FusedAdamW([p], capturable="capturable" in which, master_weights="masters" in which).step()
+    else:
+        FusedAdam([p], capturable="capturable" in which).step()
     assert p.grad._version == version
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()

@@ -811,6 +811,8 @@ template <bool Q8>
 int adamw_call(const StepCall& c, double b1, double b2, double eps, int step, uint32_t seed, const float* clip, const gsicp_adamw_device* dev, hipStream_t stream) {
     if (c.n < 0 || (c.n > 0 && (!c.params || !c.grads || !c.s0 || !c.s1 || !c.numel || !c.dtype || !c.wd))) return fail("gsicp_adamw_step: missing arrays");
     if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0)) return fail("gsicp_adamw_step: betas are in [0, 1), eps is not negative");
+    // the hardware's reciprocal takes a subnormal for zero: an element that has never had a gradient would become 0 * inf
+    if ((float)eps > 0.f && (float)eps < 0x1p-126f) return fail("gsicp_adamw_step: eps is 0 or at least 2^-126");
     if (dev) {
         if (!dev->lr_dev || !dev->step_dev || dev->bump_step < 0 || dev->bump_step > 2)
             return fail("gsicp_adamw_step: the device form needs learning rates, a step counter and bump_step 0, 1 or 2");

@@ -413,7 +413,7 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
  * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
  * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 to
  * 2^33), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap anything else it is given (checked; -2).
- * clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's clip_out), or NULL.  step: the 1-based count after the increment.
+ * eps: 0 or at least 2^-126.  clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's clip_out), or NULL.  step: the 1-based count after the increment.
  * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (live_rows and the row masks: f32
  * parameters of < 2^32 elements). */
 typedef struct {

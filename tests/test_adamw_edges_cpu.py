@@ -86,6 +86,18 @@ def test_a_step_count_of_the_host_survives_a_capture(adamw, counts):
         assert int(st["step"]) == n and bool((st["exp_avg"] == 0.5).all()) and bool((st["exp_avg_sq"] == 0.25).all())
 
 
+def test_an_eps_that_the_reciprocal_takes_for_zero_is_refused():
+    """0 / (0 + 1e-40) is 0, 0 * (1 / 1e-40) with the subnormal taken for zero would be NaN.  The pointers are never followed."""
+    from gs_icp_slam_amd import _lib
+    lib = _lib.load()
+    for name, tail in (("gsicp_adamw_step", (None, None, None)), ("gsicp_adamw_step_8bit", (0, None, None, None, None))):
+        def call(eps, n):
+            return getattr(lib, name)(n, _one(4096), _one(1 << 20), None, _one(1 << 21), _one(1 << 22), (ctypes.c_longlong * 1)(0), (ctypes.c_int * 1)(0), (ctypes.c_double * 1)(1e-3),
+                                      (ctypes.c_double * 1)(0.0), 0.9, 0.999, eps, 1, *tail)
+        for eps in (1e-40, 2.0 ** -127, 2.0 ** -149, 1.1754942e-38):
+            assert call(eps, 1) == -2 and b"eps" in lib.gsicp_last_error(), eps
+
+
 # ------------------------------------------------------------------------------------------------ state dicts of other optimisers
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("saved,loaded", [(True, True), (True, False), (False, True), (False, False)])

@@ -192,6 +192,16 @@ def test_tensors_that_are_negated_lazily_are_refused():
     assert float(m) < 0 < float(p)
 
 
+def test_the_smallest_eps_beside_elements_without_a_gradient():
+    from gs_icp_slam_amd.optim import adamw_step
+    p, g, m, v = torch.full((300,), 3.0, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+    g[::7] = 1e-3
+    adamw_step([p], [g], [m], [v], lr=0.5, step=1, eps=2.0 ** -126, weight_decay=0.0)
+    assert bool((p[g == 0] == 3.0).all()) and bool(((p[g != 0] - 2.5).abs() <= 8 * 2.0 ** -24 * 2.5).all())
+    with pytest.raises(RuntimeError, match="eps"):
+        adamw_step([p], [g], [m], [v], lr=0.5, step=2, eps=1e-40)
+
+
 # ------------------------------------------------------------------------------------------------ autograd
 @pytest.mark.parametrize("which", ["adamw_step", "adamw_step_8bit", "FusedAdamW", "FusedAdamW capturable", "FusedAdamW masters", "FusedAdam", "FusedAdam capturable"])
 def test_a_backward_over_what_a_step_has_written_is_refused(which):

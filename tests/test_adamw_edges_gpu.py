@@ -1,9 +1,10 @@
-"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture; lists; autograd."""
+"""The AdamW operators where they meet each other and the rest of the framework: clipping beside rows that are no parameters, masters under a capture; lists; autograd; types side by side."""
 import numpy as np
 import pytest
 import torch
 
 from gs_icp_slam_amd import synth
+from oracle import adamw_oracle as ao
 from tests.util import make_settings, torch_inputs
 
 pytestmark = pytest.mark.gpu
@@ -235,3 +236,110 @@ def test_a_step_over_inference_tensors():
         adamw_step(*lists, lr=0.1, step=1)
     adamw_step(*lists, lr=0.1, step=2)
     assert bool((lists[0][0] < 0.9).all())
+
+
+# ------------------------------------------------------------------------------------------------ types side by side, the device form with 16 bits and masters
+SIZES = [0, 1, 2, 7, 63, 127, 128, 129, 255, 256, 257, 1000, 2049, 5003] * 5        # more tensors than a launch takes
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+def _f64(t):
+    return t.detach().cpu().to(torch.float64).numpy()
+
+
+def _snapshot(params, grads, first, second, masters):
+    return [[None if t is None else t.detach().clone() for t in ts] for ts in (params, grads, first, second, masters)]
+
+
+def _check(before, after, bits, lr, wd, t, seed, device=False, clip=1.0):
+    """One step of every tensor against the oracle.  device: bias corrections in float32 — 1 - b^t within 8 units of 2^-24 (the rounded exponent 1, the hardware's 2^x and its argument
+    6, the difference 1), its reciprocal, the learning rate and their product 4, the reciprocal root of the other 6: 20 units of the update with all."""
+    for k, (p0, g, s0, s1, w0) in enumerate(zip(*before)):
+        n = p0.numel()
+        if n == 0:
+            continue
+        p1, n0, n1, w1 = after[0][k], after[2][k], after[3][k], after[4][k]
+        m, v = (_f64(s0), _f64(s1)) if bits == 32 else ao.decode(s0.cpu().numpy(), s1.cpu().numpy())
+        start = _f64(p0 if w0 is None else w0)
+        (P, M, V), (dp, dm, dv) = ao.step64(start, m, v, _f64(g), lr[k], wd[k], (0.9, 0.999), 1e-15, t, clip)
+        if device:
+            dp = dp + 20 * 2.0 ** -24 * np.abs(P - start * (1 - lr[k] * wd[k])) + 2.0 ** -24 * np.abs(P)
+        if bits == 32:
+            assert (np.abs(_f64(n0) - M) <= dm).all() and (np.abs(_f64(n1) - V) <= dv).all(), (t, k)
+        else:
+            codes, exps = ao.encode(*ao.step32(m, v, _f64(g), (0.9, 0.999)), *ao.random_bits(n, seed, t, k))
+            assert np.array_equal(n0.cpu().numpy().view(np.uint16), codes) and np.array_equal(n1.cpu().numpy().view(np.uint16), exps), (t, k)
+        if w0 is None:
+            assert (np.abs(_f64(p1) - P) <= dp + HALF[p1.dtype] * (np.abs(P) + dp) + TINY[p1.dtype]).all(), (t, k)
+        else:
+            assert (np.abs(_f64(w1) - P) <= dp).all() and torch.equal(w1.to(p1.dtype), p1), (t, k)
+
+
+def _grads(gen, params):
+    return [(torch.randn(p.shape, device="cuda", generator=gen) * 1e-2 * (torch.rand(p.shape, device="cuda", generator=gen) < 0.7)).to(p.dtype) for p in params]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_types_side_by_side_with_masters_for_some(bits):
+    """f32, bf16 and f16 parameters in one list, every other 16-bit one with a master."""
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, new_moments_8bit
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    dtypes = [(torch.float32, torch.bfloat16, torch.float16)[k % 3] for k in range(len(SIZES))]
+    masters = [torch.randn(n, device="cuda", generator=gen) if dt != torch.float32 and k % 2 else None for k, (n, dt) in enumerate(zip(SIZES, dtypes))]
+    params = [torch.randn(n, device="cuda", generator=gen).to(dt) if w is None else w.to(dt) for n, dt, w in zip(SIZES, dtypes, masters)]
+    if bits == 32:
+        first, second = ([torch.zeros(n, device="cuda") for n in SIZES] for _ in range(2))
+    else:
+        first, second = (list(x) for x in zip(*(new_moments_8bit(p) for p in params)))
+    lr, wd = [10.0 ** -(2 + k % 3) for k in range(len(SIZES))], [(0.0, 0.1)[k % 2] for k in range(len(SIZES))]
+    for t in (1, 2, 3):
+        grads = _grads(gen, params)
+        before = _snapshot(params, grads, first, second, masters)
+        if bits == 32:
+            adamw_step(params, grads, first, second, lr=lr, step=t, eps=1e-15, weight_decay=wd, masters=masters)
+        else:
+            adamw_step_8bit(params, grads, first, second, lr=lr, step=t, seed=21, eps=1e-15, weight_decay=wd, masters=masters)
+        _check(before, (params, grads, first, second, masters), bits, lr, wd, t, 21)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("master", [False, True])
+def test_the_device_form_with_16_bit_parameters(bits, dtype, master):
+    """Eager steps, the first of which makes the masters, then replays of one captured step with eager work between."""
+    from gs_icp_slam_amd.optim import FusedAdamW
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    params = [torch.nn.Parameter(torch.randn(n, device="cuda", generator=gen).to(dtype)) for n in SIZES]
+    groups = [{"params": params[:30], "lr": 1e-2, "weight_decay": 0.1}, {"params": params[30:], "lr": 1e-4, "weight_decay": 0.0}]
+    opt = FusedAdamW(groups, eps=1e-15, capturable=True, state_bits=bits, master_weights=master, seed=8)
+    lr, wd = [1e-2] * 30 + [1e-4] * 40, [0.1] * 30 + [0.0] * 40
+    static = [torch.zeros_like(p) for p in params]
+    for p, g in zip(params, static):
+        p.grad = g
+    names = ("exp_avg", "exp_avg_sq") if bits == 32 else ("moments", "block_exps")
+    lists = lambda: [params, static] + [[opt.state[p].get(n) for p in params] for n in names + ("master",)]       # noqa: E731
+    graph = None
+    for t in range(1, 7):
+        for g, new in zip(static, _grads(gen, params)):
+            g.copy_(new)
+        if t == 1:
+            made = [p.detach().clone() for p in params]
+            opt.step()
+            zero = [torch.zeros_like(opt.state[p][names[0]]) for p in params], [torch.zeros_like(opt.state[p][names[1]]) for p in params]
+            before = [made, static, *zero, [p.float() if master else None for p in made]]
+        else:
+            before = _snapshot(*lists())
+            if t >= 3 and graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    opt.step()
+            if t == 2 or t == 5:
+                opt.step()
+            else:
+                torch.randn(1 << 18, device="cuda").sum().item()
+                graph.replay()
+                torch.cuda.synchronize()
+        assert int(opt.state[params[0]]["step"]) == t
+        _check(before, lists(), bits, lr, wd, t, 8, device=True)

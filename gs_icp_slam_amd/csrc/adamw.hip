@@ -13,8 +13,9 @@
 // the block's scale costs no multiplication and no division.  Why STOCHASTIC rounding: with b2 = 0.999 one step moves v by a thousandth of itself, and codes are
 // 6 to 12 % apart — rounded to nearest, v would never move unless the gradient jumped eightfold; rounded up with the probability of the distance to the code
 // below, its expectation is exact.  Second moments above zero never round to zero (the smallest code instead): the denominator must not vanish; first moments below the
-// smallest code keep their expectation (that code with probability |m| / code, else zero).  As 2 * 15 exponents of v cover the same gradients as 14 of m, an element
-// at either floor still moves by at most twice the block's largest step.  Values that are not finite stay so in their own element: magnitude 127 is NaN,
+// smallest code keep their expectation (that code with probability |m| / code, else zero).  The floors fit each other: in units of the
+// bases, the element with the largest first moment has m >= 2^14 and v <= 2^31, so its step is 2^-1.5 at least, and an element at both floors has 1.125 / sqrt(1.125); below a floor an
+// element so moves by at most three times the block's largest step (eps and the end of the exponents aside).  Values that are not finite stay so in their own element: magnitude 127 is NaN,
 // second-moment code 255 is infinity.
 // The random bits are a function of (seed, step, place of the tensor in the list, element): one hashed word per 8 elements, times an odd constant per element — its
 // high and low half are the 16 bits of v and m (each uniform, because an odd multiplier permutes the words).

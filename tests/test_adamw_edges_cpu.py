@@ -1,8 +1,11 @@
-"""CPU checks of the AdamW operators at their edges: refusals of the row-aware gradient norm, optimiser state around a capture."""
+"""CPU checks of the AdamW operators at their edges: refusals of the row-aware gradient norm, optimiser state around a capture, floors of the 8-bit moments."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
+
+from oracle import adamw_oracle as ao
 
 
 def _one(*x):
@@ -204,3 +207,26 @@ def test_written_lists_raise_their_version_counters():
     for args in ((), ((b"", a),), ((b"", a), -1), ([b"", a], 1), ((b"", a), "x")):
         with pytest.raises(TypeError):
             _tensor_lists.wrote(*args)
+
+
+# ------------------------------------------------------------------------------------------------ the floors of 8-bit moments
+def test_an_element_at_a_floor_moves_by_at_most_three_times_the_largest_step():
+    """m / sqrt(v) of what the codes stand for, in blocks whose small elements have the same ratio as the large one, or any."""
+    rng = np.random.default_rng(0)
+    worst = 0.0
+    for k in range(400):
+        m, v = np.empty(128, np.float32), np.empty(128, np.float32)
+        if k < 100:                                      # the largest first moment just above a power of two, its second just below one, the rest far below
+            m[0], v[0] = 2.0 ** -5, 1.99 * 2.0 ** -9
+            scale = 2.0 ** -rng.uniform(14.5, 16.0)
+            m[1:], v[1:] = m[0] * scale, v[0] * scale ** 2
+        else:
+            m[:] = rng.choice([-1, 1], 128) * np.exp(rng.uniform(-14, 0, 128))
+            v[:] = (m.astype(np.float64) * np.exp(rng.uniform(-2, 2, 128))) ** 2
+        codes, exps = ao.encode(m, v, *ao.random_bits(128, 3, k + 1, 0))
+        a, b = ao.decode(codes, exps)
+        ratio = np.abs(a) / np.sqrt(b)
+        floor = (codes & 127 == 1) | (codes >> 8 == 1)
+        if floor.any():
+            worst = max(worst, ratio[floor].max() / ratio.max(where=~floor, initial=0.0))
+    assert 2.0 < worst <= 3.0 * (1 + 1e-12), worst

@@ -19,6 +19,8 @@
 // second-moment code 255 is infinity.
 // The random bits are a function of (seed, step, place of the tensor in the list, element): one hashed word per 8 elements, times an odd constant per element — its
 // high and low half are the 16 bits of v and m (each uniform, because an odd multiplier permutes the words).
+// Published constants: the mixer's shifts and factors (C. Wellons, "Prospecting for Hash Functions", 2018), the golden ratio (0x9E3779B1), an odd factor of A. Appleby's hashes
+// (0x85EBCA6B), the initial words of SHA-256.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -432,8 +434,8 @@ __device__ __forceinline__ void step_tile(const StepEntry& e, const Fold& f, con
     if ((threadIdx.x & 31) == 0 && (FULL || nv > 0)) ((uint16_t*)e.s1)[block] = (uint16_t)(bm | bv << 8);
 }
 
-// 1 - b^t on the device, in f32, within a few units of 2^-24 of itself: y = t ln(b) rounded once, then -(e^y - 1) by its series where that would cancel (|y| <= 0.35: the first
-// term left out is y^8 / 9! of the first), else by the hardware's 2^x
+// 1 - b^t on the device, in f32, within 8 units of 2^-24 of itself: y = t ln(b) rounded once, then -(e^y - 1) by its series where that would cancel (|y| <= 0.35: the first
+// term left out is y^8 / 9! of the first), else by the hardware's 2^x.  In f32, not by pow in double, because every wave evaluates it.
 __device__ __forceinline__ float one_minus_power(double ln_b, int t) {
     const float y = (float)fmax((double)t * ln_b, -100.0);
     constexpr float c[8] = {1.f, 1.f / 2, 1.f / 6, 1.f / 24, 1.f / 120, 1.f / 720, 1.f / 5040, 1.f / 40320};

@@ -410,12 +410,12 @@ int gsicp_adam_step_sparse(int n_groups, float* const* params, const float* cons
  * torch.optim.AdamW's step (amsgrad, maximize off) over any number of tensors, 64 per launch (56 in the device form):
  *     g' = *clip g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;
  *     p = (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
- * All arithmetic in f32, bias corrections in double.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
+ * All arithmetic in f32; the bias corrections in double, or in f32 within 8 units of 2^-24 in the device form.  HOST arrays of n entries: DEVICE pointers params / grads (dtype[k]: 0 f32, 1 bf16, 2 f16, the same for both), masters
  * (f32 copy that takes the update, the parameter receives it rounded; NULL array or NULL entry: none; 16-bit parameters only), exp_avg / exp_avg_sq (f32), numel (0 to
  * 2^33), lr, weight_decay.  Pointers need the alignment of their element only.  What the call writes must not overlap anything else it is given (checked; -2).
  * eps: 0 or at least 2^-126.  clip: DEVICE float, the factor of every gradient (gsicp_grad_norm's clip_out), or NULL.  step: the 1-based count after the increment.
- * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (live_rows and the row masks: f32
- * parameters of < 2^32 elements). */
+ * dev: NULL, or the DEVICE form (lr and step are then ignored) for a captured graph; its fields mean what they mean in gsicp_adam_step_sparse (the row masks: f32 parameters of
+ * < 2^32 elements; live_rows: any). */
 typedef struct {
     const double* lr_dev;              /* DEVICE double[n] */
     int* step_dev;                     /* DEVICE int: steps taken so far */

@@ -349,6 +349,9 @@ def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, 
                                                      masters)
         mast, numels = at + 32 * n, at + 40 * n
     codes = numels + 8 * n
+    step = int(step)
+    if step > 0x7FFFFFFF:                       # the call below would take its low 32 bits
+        raise RuntimeError(f"{what}: a step count has 31 bits")
     weight_decay = _doubles(what, "weight_decay", weight_decay, n)
     if device_form is None:
         lr, dev, dev_keep = _doubles(what, "lr", lr, n), None, None
@@ -358,7 +361,7 @@ def _adamw(what, bits, params, grads, masters, first, second, lr, weight_decay, 
     if clip is None and max_norm is not None:
         norm, buffer = _norm(what, device, current, stream, n, at + 8 * n, numels, codes, max_norm)
         clip = buffer.data_ptr()
-    args = (n, at, at + 8 * n, mast, at + 16 * n, at + 24 * n, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, int(step))
+    args = (n, at, at + 8 * n, mast, at + 16 * n, at + 24 * n, numels, codes, _at(lr), _at(weight_decay), betas[0], betas[1], eps, step)
     if bits == 32:
         _call("gsicp_adamw_step", device, current, *args, clip, dev, stream)
     else:

@@ -203,6 +203,18 @@ def test_the_smallest_eps_beside_elements_without_a_gradient():
         adamw_step([p], [g], [m], [v], lr=0.5, step=2, eps=1e-40)
 
 
+@pytest.mark.parametrize("step", [1 << 31, (1 << 32) + 1, 1 << 40, 0, -1])
+def test_step_counts_that_do_not_fit_are_refused(step):
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, new_moments_8bit
+    lists = [[torch.ones(5, device="cuda")] for _ in range(4)]
+    with pytest.raises(RuntimeError, match="step"):
+        adamw_step(*lists, lr=0.1, step=step)
+    m, x = new_moments_8bit(lists[0][0])
+    with pytest.raises(RuntimeError, match="step"):
+        adamw_step_8bit(*lists[:2], [m], [x], lr=0.1, step=step)
+    assert all(bool((t[0] == 1).all()) for t in lists)
+
+
 # ------------------------------------------------------------------------------------------------ autograd
 @pytest.mark.parametrize("which", ["adamw_step", "adamw_step_8bit", "FusedAdamW", "FusedAdamW capturable", "FusedAdamW masters", "FusedAdam", "FusedAdam capturable"])
 def test_a_backward_over_what_a_step_has_written_is_refused(which):

@@ -355,3 +355,68 @@ def test_the_device_form_with_16_bit_parameters(bits, dtype, master):
                 torch.cuda.synchronize()
         assert int(opt.state[params[0]]["step"]) == t
         _check(before, lists(), bits, lr, wd, t, 8, device=True)
+
+
+# ------------------------------------------------------------------------------------------------ the functions in a graph, large gathers
+def test_the_functions_in_one_captured_graph():
+    """Norm, clipped 8-bit and 32-bit step, values and rows of the moments: replays against the same calls made eagerly, with eager work between."""
+    from gs_icp_slam_amd.optim import adamw_step, adamw_step_8bit, decode_moments, gather_moments_8bit, grad_norm
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    shapes = [(2001, 3), (2001, 45), (2001, 1)]
+    start = [torch.randn(s, device="cuda", generator=gen) for s in shapes]
+    index = torch.randint(-1, 2001, (1500,), device="cuda", generator=gen)
+
+    def state():
+        f32 = lambda: [torch.zeros(s, device="cuda") for s in shapes]      # noqa: E731
+        return dict(p=[t.clone() for t in start], q=[t.clone() for t in start], g=f32(), m=f32(), v=f32(), c=[torch.zeros(s, dtype=torch.int16, device="cuda") for s in shapes],
+                    x=[torch.zeros(-(-t.numel() // 128), dtype=torch.int16, device="cuda") for t in start])
+
+    def run(s):
+        n0 = grad_norm(s["g"])
+        n1 = adamw_step_8bit(s["p"], s["g"], s["c"], s["x"], lr=1e-2, step=7, seed=3, max_norm=0.3)
+        n2 = adamw_step(s["q"], s["g"], s["m"], s["v"], lr=1e-2, step=7, max_norm=0.3)
+        m, v = decode_moments(s["c"], s["x"])
+        gc, gx = gather_moments_8bit(s["c"], s["x"], index)
+        return [n0, n1, n2, *m, *v, *gc, *gx]
+    a, b = state(), state()
+    run(b)                                       # loads the kernels
+    b = state()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(b)
+    for k in range(5):
+        for g, h in zip(a["g"], b["g"]):
+            g.copy_(torch.randn(g.shape, device="cuda", generator=gen))
+            h.copy_(g)
+        want = run(a)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(want, out)), k
+        assert all(torch.equal(x, y) for name in a for x, y in zip(a[name], b[name])), k
+
+
+def test_gathered_rows_past_two_to_the_31():
+    """As many elements as a gather takes (2^32 - 1 less what is missing to a whole row), the first and last blocks and those around 2^31."""
+    from gs_icp_slam_amd.optim import gather_moments_8bit
+    w = 3
+    rows = (1 << 32) // w                                    # 2^32 - 1 elements
+    rng = np.random.default_rng(0)
+    n = rows * w
+    windows = [0, (1 << 31) // 384 * 384, (n - 384) // 384 * 384]
+    c = torch.zeros(n, dtype=torch.int16, device="cuda")
+    x = torch.zeros(-(-n // 128), dtype=torch.int16, device="cuda")
+    want = []
+    for at in windows:
+        codes, exps = ao.encode(rng.normal(size=384).astype(np.float32), rng.normal(size=384).astype(np.float32) ** 2, *ao.random_bits(384, 1, 1, 0))
+        c[at: at + 384] = torch.from_numpy(codes.view(np.int16)).cuda()
+        x[at // 128: at // 128 + 3] = torch.from_numpy(exps.view(np.int16)).cuda()
+        want.append(ao.gather(codes, exps, w, np.arange(128), 128))
+    index = torch.arange(rows, device="cuda")
+    (oc,), (ox,) = gather_moments_8bit([c.view(rows, w)], [x], index)
+    oc = oc.view(-1)
+    for at, (codes, exps) in zip(windows, want):
+        assert np.array_equal(oc[at: at + 384].cpu().numpy().view(np.uint16), codes), at
+        assert np.array_equal(ox[at // 128: at // 128 + 3].cpu().numpy().view(np.uint16), exps), at
+    assert sum(int((t != 0).sum()) for t in oc.split(1 << 28)) == sum(int((codes != 0).sum()) for codes, _ in want)
+    with pytest.raises(RuntimeError):
+        gather_moments_8bit([c.view(rows, w)], [x], torch.arange(rows + 1, device="cuda"))

@@ -30,6 +30,20 @@ from . import _lib
 _MAX = 8
 
 
+def _counts_beside(step, p):
+    """Whether a state's step count is what the capturable kernels read and advance: an int32 tensor on the parameter's device."""
+    return torch.is_tensor(step) and step.dtype == torch.int32 and step.device == p.device
+
+
+def _counter_beside(step, p, made):
+    """A step count as that, wherever and whatever it was (a number, a tensor of a state that was loaded to the host, torch's float counter).  made: what the call has made so far;
+    counters that were one tensor stay one, of others those that agree become one."""
+    key = (step.data_ptr() if torch.is_tensor(step) and step.dtype == torch.int32 else int(step), p.device)
+    if key not in made:
+        made[key] = torch.full((), int(step), dtype=torch.int32, device=p.device)
+    return made[key]
+
+
 class FusedAdam(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, capturable=False):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
@@ -58,7 +72,7 @@ class FusedAdam(torch.optim.Optimizer):
         for group in self.param_groups:
             for p in group["params"]:
                 st = self.state.get(p, {})
-                if not torch.is_tensor(st.get("step")):
+                if not _counts_beside(st.get("step"), p):
                     return None
                 steps[st["step"].data_ptr()] = st["step"]
         return next(iter(steps.values())) if len(steps) == 1 else None
@@ -126,7 +140,7 @@ class FusedAdam(torch.optim.Optimizer):
         # a map store re-binds fresh Parameter objects into the same groups [REF scene/gaussian_model.py:409-492] (ids of dead objects
         # can be reused by CPython, group positions cannot)
         buckets = {}
-        fresh = {}
+        fresh, moved = {}, {}
         for gi, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             for pi, p in enumerate(group["params"]):
@@ -143,6 +157,8 @@ class FusedAdam(torch.optim.Optimizer):
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 elif not torch.is_tensor(st["step"]):
                     st["step"] = torch.full((), int(st["step"]), dtype=torch.int32, device=p.device)
+                elif not _counts_beside(st["step"], p):
+                    st["step"] = _counter_beside(st["step"], p, moved)
                 buckets.setdefault((float(b1), float(b2), float(group["eps"]), st["step"].data_ptr()), []).append(
                     (p, p.grad, st["exp_avg"], st["exp_avg_sq"], float(group["lr"]), st["step"], (gi, pi)))
         capturing = torch.cuda.is_current_stream_capturing()
@@ -515,9 +531,8 @@ class FusedAdamW(FusedAdam):
         for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
             for k, v in state_dict["state"].get(i, {}).items():
                 if k == "step":
-                    key = (v.data_ptr() if torch.is_tensor(v) and v.dtype == torch.int32 else int(v), p.device)      # torch's optimisers: a counter per parameter
                     if self.capturable:
-                        v = steps.setdefault(key, torch.full((), int(v), dtype=torch.int32, device=p.device))
+                        v = _counter_beside(v, p, steps)
                     else:
                         v = int(v)
                 elif torch.is_tensor(v):
@@ -550,7 +565,7 @@ class FusedAdamW(FusedAdam):
                 loss = closure()
         if step_already_bumped and not self.capturable:
             raise RuntimeError("FusedAdamW.step(step_already_bumped=True) needs capturable=True (a device step counter)")
-        buckets, fresh, place, may_run = {}, {}, -1, self.capturable
+        buckets, fresh, moved, place, may_run = {}, {}, {}, -1, self.capturable
         for gi, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             for pi, p in enumerate(group["params"]):
@@ -566,14 +581,14 @@ class FusedAdamW(FusedAdam):
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW: sparse gradients are not supported")
                 st = self.state[p]
-                if self.capturable and not torch.is_tensor(st.get("step")) and torch.cuda.is_current_stream_capturing():      # state made now would live in the graph, unwritten
+                if self.capturable and not _counts_beside(st.get("step"), p) and torch.cuda.is_current_stream_capturing():      # state made now would live in the graph, unwritten
                     raise RuntimeError("FusedAdamW(capturable): run one step() outside graph capture first (allocates the state)")
                 if not st:
                     if self.capturable and p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.int32, device=p.device)
                     self._new_state(p, fresh[p.device] if self.capturable else 0)
-                elif self.capturable and not torch.is_tensor(st["step"]):
-                    st["step"] = fresh.setdefault((int(st["step"]), p.device), torch.full((), int(st["step"]), dtype=torch.int32, device=p.device))
+                elif self.capturable and not _counts_beside(st["step"], p):
+                    st["step"] = _counter_beside(st["step"], p, moved)
                 key = (float(b1), float(b2), float(group["eps"]), st["step"].data_ptr() if self.capturable else int(st["step"]), p.device)
                 buckets.setdefault(key, []).append((p, p.grad.contiguous(), st, gi, pi, place))
         clip = buffer = None

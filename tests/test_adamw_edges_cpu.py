@@ -192,6 +192,28 @@ def test_counts_of_a_torch_optimiser_that_agree_share_one_device_counter():
     assert counters[0] == counters[1] != counters[2] == counters[3]
 
 
+@pytest.mark.parametrize("cls", ["FusedAdam", "FusedAdamW"])
+def test_counters_elsewhere_are_not_handed_to_a_kernel(cls):
+    """A state loaded to the host, or with torch's float counters: its address is not one that the loss kernel or the step may advance."""
+    from gs_icp_slam_amd import optim
+    params = [torch.nn.Parameter(torch.ones(3, device="meta")) for _ in range(3)]
+    opt = getattr(optim, cls)(params, capturable=True)
+    there = torch.zeros((), dtype=torch.int32, device="meta")
+    for step, taken in ((there, True), (torch.zeros((), dtype=torch.int32), False), (torch.zeros((), device="meta"), False), (torch.tensor(4.0), False), (4, False)):
+        for p in params:
+            opt.state[p]["step"] = step
+        assert (opt.shared_step_tensor() is there) == taken, step
+        assert all(optim._counts_beside(opt.state[p]["step"], p) == taken for p in params)
+    host = torch.full((), 6, dtype=torch.int32)
+    q = torch.nn.Parameter(torch.ones(3, dtype=torch.float64))
+    made = {}
+    a, b = optim._counter_beside(host, params[0], made), optim._counter_beside(host, params[1], made)
+    assert a is b and a.dtype == torch.int32 and a.device.type == "meta"
+    assert optim._counter_beside(host.clone(), params[0], made) is not a                       # another counter that agrees by chance
+    c = [optim._counter_beside(x, q, made) for x in (6, torch.tensor(6.0), 7)]
+    assert c[0] is c[1] is not c[2] and [int(x) for x in c] == [6, 6, 7]
+
+
 # ------------------------------------------------------------------------------------------------ lists of tensors
 def test_written_lists_raise_their_version_counters():
     from gs_icp_slam_amd import _tensor_lists

@@ -357,6 +357,40 @@ def test_the_device_form_with_16_bit_parameters(bits, dtype, master):
         _check(before, lists(), bits, lr, wd, t, 8, device=True)
 
 
+@pytest.mark.parametrize("cls", ["FusedAdam", "FusedAdamW"])
+@pytest.mark.parametrize("counter", ["int32 on the host", "float32 on the host", "float32 beside", "number"])
+def test_a_state_whose_counter_is_elsewhere_continues(cls, counter, tmp_path):
+    """Checkpoints are loaded to the host, torch's optimisers count in float32: the capturable step moves the counter beside the parameter and goes on."""
+    from gs_icp_slam_amd import optim
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    start = [torch.randn(n, device="cuda", generator=gen) for n in (5, 300, 4001)]
+    feeds = [[torch.randn(p.shape, device="cuda", generator=gen) for p in start] for _ in range(4)]
+
+    def go(opt, params, ks):
+        for k in ks:
+            for p, g in zip(params, feeds[k]):
+                p.grad = g.clone()
+            opt.step()
+    a_p = [torch.nn.Parameter(p.clone()) for p in start]
+    a = getattr(optim, cls)(a_p, lr=1e-2, capturable=True)
+    go(a, a_p, (0, 1))
+    torch.save(a.state_dict(), tmp_path / "s.pt")
+    state = torch.load(tmp_path / "s.pt", map_location="cpu" if "host" in counter else "cuda", weights_only=True)
+    b_p = [torch.nn.Parameter(p.detach().clone()) for p in a_p]
+    b = getattr(optim, cls)(b_p, lr=1e-2, capturable=True)
+    b.load_state_dict(state)
+    for p in b_p:
+        st = b.state[p]
+        st["step"] = {"int32 on the host": torch.full((), 2, dtype=torch.int32), "float32 on the host": torch.tensor(2.0), "float32 beside": torch.tensor(2.0, device="cuda"),
+                      "number": 2}[counter]
+    assert b.shared_step_tensor() is None
+    go(a, a_p, (2, 3))
+    go(b, b_p, (2, 3))
+    for p, q in zip(a_p, b_p):
+        assert torch.equal(p, q) and torch.equal(a.state[p]["exp_avg_sq"], b.state[q]["exp_avg_sq"])
+        assert b.state[q]["step"].device == q.device and b.state[q]["step"].dtype == torch.int32 and int(b.state[q]["step"]) == 4
+
+
 # ------------------------------------------------------------------------------------------------ the functions in a graph, large gathers
 def test_the_functions_in_one_captured_graph():
     """Norm, clipped 8-bit and 32-bit step, values and rows of the moments: replays against the same calls made eagerly, with eager work between."""

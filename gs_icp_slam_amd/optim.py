@@ -149,6 +149,8 @@ class FusedAdam(torch.optim.Optimizer):
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous() or not p.grad.is_contiguous():
                     raise RuntimeError("FusedAdam(capturable): parameters and gradients must be contiguous float32 on the HIP device")
                 st = self.state[p]
+                if not _counts_beside(st.get("step"), p) and torch.cuda.is_current_stream_capturing():      # state made now would live in the graph, unwritten
+                    raise RuntimeError("FusedAdam(capturable): run one step() outside graph capture first (allocates the state)")
                 if len(st) == 0:
                     if p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.int32, device=p.device)
@@ -581,7 +583,7 @@ class FusedAdamW(FusedAdam):
                 if p.grad.is_sparse:
                     raise RuntimeError("FusedAdamW: sparse gradients are not supported")
                 st = self.state[p]
-                if self.capturable and not _counts_beside(st.get("step"), p) and torch.cuda.is_current_stream_capturing():      # state made now would live in the graph, unwritten
+                if self.capturable and not _counts_beside(st.get("step"), p) and torch.cuda.is_current_stream_capturing():      # as in FusedAdam
                     raise RuntimeError("FusedAdamW(capturable): run one step() outside graph capture first (allocates the state)")
                 if not st:
                     if self.capturable and p.device not in fresh:

@@ -391,6 +391,34 @@ def test_a_state_whose_counter_is_elsewhere_continues(cls, counter, tmp_path):
         assert b.state[q]["step"].device == q.device and b.state[q]["step"].dtype == torch.int32 and int(b.state[q]["step"]) == 4
 
 
+@pytest.mark.parametrize("first_steps", [0, 2])
+def test_a_refused_capture_leaves_fused_adam_as_it_was(first_steps):
+    """Neither a first step nor the first one after host step counts can be captured; an eager step afterwards starts from where the state stood."""
+    from gs_icp_slam_amd.optim import FusedAdam
+    start = [torch.ones(n, device="cuda") for n in (5, 700)]
+    host, dev = ([torch.nn.Parameter(p.clone()) for p in start] for _ in range(2))
+    a, b = FusedAdam(host, lr=1e-2), FusedAdam(dev, lr=1e-2, capturable=True)
+    for p in host:
+        p.grad = torch.full_like(p, 0.5)
+    for _ in range(first_steps):
+        a.step()
+    for p, q in zip(host, dev):
+        q.data.copy_(p)
+        q.grad = p.grad.clone()
+        if first_steps:
+            b.state[q].update({n: v.clone() if torch.is_tensor(v) else v for n, v in a.state[p].items()})
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="outside graph capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.step()
+    assert all(b.state[q].get("step", 0) == first_steps for q in dev)
+    a.step()
+    b.step()
+    for p, q in zip(host, dev):
+        assert torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"]) and torch.equal(a.state[p]["exp_avg_sq"], b.state[q]["exp_avg_sq"])
+        assert int(b.state[q]["step"]) == first_steps + 1 == a.state[p]["step"]
+
+
 # ------------------------------------------------------------------------------------------------ the functions in a graph, large gathers
 def test_the_functions_in_one_captured_graph():
     """Norm, clipped 8-bit and 32-bit step, values and rows of the moments: replays against the same calls made eagerly, with eager work between."""

@@ -651,17 +651,19 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
     }
     return s;
 }
-// the same of an f32 tensor of less than 2^32 elements without its frozen rows
+// The same of an f32 tensor of less than 2^32 elements without its frozen rows; FULL: the whole tile exists.  4.2 M elements of 300 k rows: 8.9 us with half of the rows frozen, 5.8
+// with a live count only, 5.6 as they are.
+template <bool FULL>
 __device__ __forceinline__ double norm_frozen_tile(const NormEntry& e, const Rows& rows, uint32_t tile, int lanes, int lane) {
     double s = 0.0;
-#pragma unroll 1
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
         const long long at = (long long)tile * (16 * lanes) + 4 * (k * lanes + lane);
-        const int nv = (int)max(0ll, min(4ll, e.numel - at));
-        if (nv == 0) break;
+        const int nv = FULL ? 4 : (int)max(0ll, min(4ll, e.numel - at));
+        if (!FULL && nv == 0) break;
         float x[4];
         uint32_t row[4];
-        load4<F32, false, false>(e.g, at, nv, x);
+        load4<F32, FULL, false>(e.g, at, nv, x);
         rows.of4((uint32_t)at, nv, row);
         const uint32_t moves = rows.width >= 3u ? flags2(rows.freeze, row, 1) : flags4(rows.freeze, row, 1);
 #pragma unroll
@@ -681,7 +683,10 @@ __device__ __forceinline__ double norm_any_tile(const NormTable<ROWS>& t, uint32
         const uint32_t w = t.row_width[k];
         if (t.live_rows && w > 0) e.numel = min(e.numel, (long long)*t.live_rows * w);
         if ((long long)mine * norm_tile_elems(e.dtype, 64 * lanes) >= e.numel) return 0.0;
-        if (e.frozen) return norm_frozen_tile(e, {w, t.row_magic[k], row_shift(w), nullptr, t.row_freeze}, mine, lanes, lane);
+        if (e.frozen) {
+            const Rows rows = {w, t.row_magic[k], row_shift(w), nullptr, t.row_freeze};
+            return ((long long)mine + 1) * (16 * lanes) <= e.numel ? norm_frozen_tile<true>(e, rows, mine, lanes, lane) : norm_frozen_tile<false>(e, rows, mine, lanes, lane);
+        }
     }
     return e.dtype == F32 ? norm_tile<F32, NT>(e, mine, lanes, lane) : e.dtype == BF16 ? norm_tile<BF16, NT>(e, mine, lanes, lane) : norm_tile<F16, NT>(e, mine, lanes, lane);
 }

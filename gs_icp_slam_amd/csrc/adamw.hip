@@ -46,7 +46,8 @@ constexpr long long MAX_NUMEL = 1ll << 33;   // 2^25 workgroups of the step for 
 constexpr unsigned long long STEP_TILES = (1u << 26) - 1, DECODE_TILES = (1u << 24) - 1;
 constexpr int TILE_ELEMS = 256;       // elements of a workgroup of the step and of the gathering: ONE wave, four consecutive elements a lane, no loop
 constexpr int NORM_GRID = 2048;       // partial sums of one norm launch
-constexpr int NORM_SMALL_TILES = 64;  // 4 KB tiles that one workgroup of 16 waves takes by itself: 64 of them 7.4 us against 10.9 in two launches, 128 12.3 against 10.8
+constexpr int NORM_SMALL_TILES = 64;  // 4 KB tiles that one workgroup of 16 waves takes by itself: 64 of them 7.4 us against 10.9 in two launches, 128 12.3 against 10.8 (they are
+                                      // even somewhere between: 64 is on the safe side, not the crossing itself)
 constexpr int QBLOCK = 128;           // elements per base exponent: 32 lanes x 4
 
 enum Dtype { F32 = 0, BF16 = 1, F16 = 2 };
@@ -449,8 +450,8 @@ __device__ __forceinline__ float one_minus_power(double ln_b, int t) {
 // device memory (a captured graph replays them).
 // Measured: 236 M f32 parameters, 32-bit moments 1.08 ms = 6.1 TB/s (a copy written the same way 6.5; a grid-stride loop of 2 048 workgroups of 256 lanes 1.34 ms, one tile of
 // 2 048 elements a workgroup 1.26, of 1 024 1.10 - 1.14); 140 M with 8-bit moments 0.345 ms = 6.5 TB/s (with the correctly rounded root and quotient and 108 instructions an
-// element 0.382: bound by them); 560 k parameters 4.1 us, 608 in 64 tensors 3.5 us: a launch.  The captured iteration's 4.2 M parameters of 300 k rows, radii mask: 20.8 us,
-// 8-bit 17.4.
+// element 0.382: bound by them); 560 k parameters 4.1 us, 608 in 64 tensors 3.5 us: a launch.  The device form on 4.2 M parameters of 300 k rows: 19.2 us,
+// with a radii mask 20.3; 8-bit 13.8 and 15.5.
 template <bool Q8, bool DEV, bool MASKED, bool NT>
 __global__ __launch_bounds__(64) void adamw_step_kernel(StepTable<DEV> t, StepHyper h) {
     const uint32_t tile = blockIdx.x, k = find_tensor(t.first, tile), mine = tile - t.first[k];
@@ -652,7 +653,7 @@ __device__ __forceinline__ double norm_tile(const NormEntry& e, uint32_t tile, i
     return s;
 }
 // The same of an f32 tensor of less than 2^32 elements without its frozen rows; FULL: the whole tile exists.  4.2 M elements of 300 k rows: 8.9 us with half of the rows frozen, 5.8
-// with a live count only, 5.6 as they are.
+// with a live count only, 5.0 as they are.
 template <bool FULL>
 __device__ __forceinline__ double norm_frozen_tile(const NormEntry& e, const Rows& rows, uint32_t tile, int lanes, int lane) {
     double s = 0.0;
